@@ -437,6 +437,59 @@ ttc_status ttc_float_to_int16(ttc_ctx* ctx, const float* d_in, int64_t n, float 
  * median, convert_to_db(., 22) (job.py:74-89).  d_u16 [T, X, Y, 2] -> d_out [T, X, Y, 2] float32. */
 ttc_status ttc_s1_to_db(ttc_ctx* ctx, const uint16_t* d_u16, int32_t T, int32_t X, int32_t Y, float* d_out, void* stream);
 
+/* ---- channels-last layer operators -----------------------------------------------------------------------------------------------
+ * The two layers a head on the exported features (ttc_forward_taps: early / late [n, H, W, 64], channels last) is made of, on arrays of
+ * the caller's own sizes, forward and backward:
+ *   ttc_group_norm  group norm with an activation   (the graph's layer: src/train/src/model.py:100-121, followed by sigmoid / tanh in
+ *                   the ConvGRU cell, :259-285)
+ *   ttc_linear      y = residual + scale * act(x w + bias): a 1x1 convolution = the product of every pixel's channels with w [cin, cout]
+ *                   (TF layout [1, 1, cin, cout]); the graph's 1x1 sigmoid head (src/train/train-model.py:226-231) is
+ *                   linear(late, head/kernel, head/bias, sigmoid)
+ * Arrays are fp32, fp16 or bf16 (one type per call); gamma, beta, bias, the statistics and the gradients of gamma, beta and bias are always
+ * float32.  Sums and statistics are held in 32 bits or more, results are rounded once; no atomics: two runs give the same bits.
+ * Nothing here uses the context's workspace, weights or window geometry: the caller passes the scratch memory the *_workspace query
+ * names (16-byte aligned), so calls on several streams and calls captured into several graphs do not share any.  No call allocates, synchronises or
+ * copies; all of them can be captured into a graph.  Rows need unit channel stride and may be a slice of wider rows; a row may start at any
+ * element.  Outputs are contiguous and must not overlap inputs.  n = 0 or rows = 0 is a valid call. */
+enum { TTC_DT_F32 = 0, TTC_DT_F16 = 2, TTC_DT_BF16 = 3 };       /* the codes of ttc_config.precision */
+enum { TTC_ACT_NONE = 0, TTC_ACT_RELU = 1, TTC_ACT_SWISH = 2, TTC_ACT_SIGMOID = 3, TTC_ACT_TANH = 4, TTC_ACT_GELU = 5 };   /* GELU: erf form */
+
+typedef struct {
+    int32_t dtype, activation;
+    int64_t n, rows;             /* samples (<= 65535), pixels per sample: statistics span rows x (channels / groups)             */
+    int32_t channels, groups;    /* groups divides channels <= 4096                                                               */
+    int64_t x_stride, x_pitch;   /* elements between samples / rows of x                                                          */
+    float   eps;                 /* >= 0, added to the biased variance (1e-5 in the graph)                                        */
+} ttc_group_norm_desc;
+ttc_status ttc_group_norm_workspace(const ttc_group_norm_desc* desc, int32_t backward, size_t* bytes);
+/* d_y [n, rows, channels] = act(gamma * (x - mean) / sqrt(var + eps) + beta); d_gamma / d_beta [channels], NULL = 1 / 0;
+ * d_stats [n, groups, 2] float32 = (mean, 1 / sqrt(var + eps)) for the backward pass, may be NULL. */
+ttc_status ttc_group_norm(ttc_ctx* ctx, const ttc_group_norm_desc* desc, const void* d_x, const float* d_gamma, const float* d_beta,
+                          void* d_y, float* d_stats, void* d_ws, size_t ws_bytes, void* stream);
+/* gradients of ttc_group_norm for d_dy (strides as x's, of its own): d_dx [n, rows, channels], d_dgamma / d_dbeta [channels] float32; each may be NULL.
+ * With n = 0 or rows = 0 the parameter gradients are written as 0. */
+ttc_status ttc_group_norm_backward(ttc_ctx* ctx, const ttc_group_norm_desc* desc, const void* d_dy, int64_t dy_stride, int64_t dy_pitch,
+                                   const void* d_x, const float* d_gamma, const float* d_beta, const float* d_stats, void* d_dx,
+                                   float* d_dgamma, float* d_dbeta, void* d_ws, size_t ws_bytes, void* stream);
+
+typedef struct {
+    int32_t dtype, activation;
+    int64_t rows;                /* pixels                                                                                        */
+    int32_t cin, cout;           /* 1 .. 65536                                                                                    */
+    int64_t x_pitch, w_pitch;    /* elements between rows of x and of w                                                           */
+    int64_t res_pitch, dy_pitch; /* of the residual (ttc_linear) / of dy (ttc_linear_backward)                                    */
+    float   scale;               /* y = residual + scale * act(x w + bias): 0.1 in DSen2's residual blocks, else 1                */
+} ttc_linear_desc;
+ttc_status ttc_linear_workspace(const ttc_linear_desc* desc, int32_t backward, size_t* bytes);
+/* d_y [rows, cout]; d_bias [cout] and d_residual [rows, cout] may be NULL; d_preact [rows, cout] (the type of x, may be NULL) receives
+ * x w + bias for the backward pass. */
+ttc_status ttc_linear(ttc_ctx* ctx, const ttc_linear_desc* desc, const void* d_x, const void* d_w, const float* d_bias, const void* d_residual,
+                      void* d_y, void* d_preact, void* d_ws, size_t ws_bytes, void* stream);
+/* gradients of ttc_linear: with dz = scale * dy * act'(preact), d_dx [rows, cin] = dz w^T, d_dw [cin, cout] = x^T dz (0 for rows = 0),
+ * d_dbias [cout] float32 = column sums of dz; each may be NULL.  The residual's gradient is dy.  d_preact: needed with an activation. */
+ttc_status ttc_linear_backward(ttc_ctx* ctx, const ttc_linear_desc* desc, const void* d_dy, const void* d_x, const void* d_w,
+                               const void* d_preact, void* d_dx, void* d_dw, float* d_dbias, void* d_ws, size_t ws_bytes, void* stream);
+
 /* ---- on-disk formats (host code, no GPU) ----------------------------------------------------------------------------------
  * hkl.load(path) for the numeric arrays of temp/raw (src/download_and_predict_job.py:684-714; written at :462-463, :592-633
  * with hkl.dump(..., compression='gzip')): reads the dataset at `name`, a '/'-separated path from the root ("data",

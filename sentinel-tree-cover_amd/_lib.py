@@ -26,6 +26,7 @@ EXPORTS = [
     "ttc_border_subtiles", "ttc_seam_adjust", "ttc_reseg_mosaic", "ttc_smooth_strip", "ttc_superresolve_windows", "ttc_count_equal", "ttc_write_geotiff_u8",
     "ttc_predict_tile", "ttc_read_hkl", "ttc_read_hkl_error",
     "ttc_create_v2", "ttc_predict_tile_shaped", "ttc_adjust_shape", "ttc_debug_kernel_flops", "ttc_calibrate_precision",
+    "ttc_group_norm_workspace", "ttc_group_norm", "ttc_group_norm_backward", "ttc_linear_workspace", "ttc_linear", "ttc_linear_backward",
 ]
 
 # exported for tools/probes and the detector-stage tests, declared in csrc/ttc_internal.h -- not part of the drop-in surface (include/ttc.h)
@@ -67,6 +68,21 @@ class TTCPrecisionReport(C.Structure):
 class TTCResegWindow(C.Structure):
     _fields_ = [("kind", C.c_int32), ("x", C.c_int32), ("y", C.c_int32), ("rows", C.c_int32), ("cols", C.c_int32),
                 ("pred_off", C.c_int64), ("weight_off", C.c_int64)]
+
+
+class TTCGroupNormDesc(C.Structure):
+    """ttc_group_norm_desc"""
+    _fields_ = [("dtype", C.c_int32), ("activation", C.c_int32), ("n", C.c_int64), ("rows", C.c_int64), ("channels", C.c_int32),
+                ("groups", C.c_int32), ("x_stride", C.c_int64), ("x_pitch", C.c_int64), ("eps", C.c_float)]
+
+
+class TTCLinearDesc(C.Structure):
+    """ttc_linear_desc"""
+    _fields_ = [("dtype", C.c_int32), ("activation", C.c_int32), ("rows", C.c_int64), ("cin", C.c_int32), ("cout", C.c_int32),
+                ("x_pitch", C.c_int64), ("w_pitch", C.c_int64), ("res_pitch", C.c_int64), ("dy_pitch", C.c_int64), ("scale", C.c_float)]
+
+
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "swish": 2, "sigmoid": 3, "tanh": 4, "gelu": 5}     # TTC_ACT_*
 
 
 class TTCTensor(C.Structure):
@@ -156,6 +172,13 @@ def load():
     lib.ttc_debug_check_guards.argtypes = [P, C.POINTER(C.c_int64), C.c_char_p, C.c_size_t]
     lib.ttc_debug_kernel_ms.argtypes = [P, C.c_char_p, C.POINTER(C.c_double), C.POINTER(C.c_int64)]
     lib.ttc_debug_kernel_flops.argtypes = [P, C.c_char_p, C.POINTER(C.c_double), C.POINTER(C.c_int64)]
+    SZ, GN, LN = C.c_size_t, C.POINTER(TTCGroupNormDesc), C.POINTER(TTCLinearDesc)
+    lib.ttc_group_norm_workspace.argtypes = [GN, I32, C.POINTER(SZ)]
+    lib.ttc_group_norm.argtypes = [P, GN, VP, VP, VP, VP, VP, VP, SZ, VP]
+    lib.ttc_group_norm_backward.argtypes = [P, GN, VP, C.c_int64, C.c_int64, VP, VP, VP, VP, VP, VP, VP, VP, SZ, VP]
+    lib.ttc_linear_workspace.argtypes = [LN, I32, C.POINTER(SZ)]
+    lib.ttc_linear.argtypes = [P, LN, VP, VP, VP, VP, VP, VP, VP, SZ, VP]
+    lib.ttc_linear_backward.argtypes = [P, LN, VP, VP, VP, VP, VP, VP, VP, VP, SZ, VP]
     for name in EXPORTS:
         fn = getattr(lib, name)          # AttributeError here == missing export
         if name not in ("ttc_version", "ttc_destroy", "ttc_last_error", "ttc_device_bytes", "ttc_read_hkl_error"):
@@ -223,6 +246,73 @@ def pack_tensors(weights: dict):
         for d in range(min(a.ndim, 4)):
             arr[i].shape[d] = a.shape[d]
     return arr, keep
+
+
+_fns = None
+
+
+def _layer_functions():
+    """the torch.autograd functions of Context.group_norm / Context.linear (torch is imported on first use)"""
+    global _fns
+    if _fns is not None:
+        return _fns
+    import torch
+    from torch.autograd.function import once_differentiable
+
+    class GroupNorm(torch.autograd.Function):
+        @staticmethod
+        def forward(fctx, lib_ctx, x, gamma, beta, groups, eps, activation):
+            y, stats = lib_ctx._group_norm(x, gamma, beta, groups, eps, activation, True)
+            fctx.save_for_backward(x, gamma, beta, stats)
+            fctx.lib_ctx, fctx.activation = lib_ctx, activation
+            return y
+
+        @staticmethod
+        @once_differentiable
+        def backward(fctx, dy):
+            x, gamma, beta, stats = fctx.saved_tensors
+            _, nx, ng, nb = fctx.needs_input_grad[:4]
+            dx, dg, db = fctx.lib_ctx.group_norm_backward(dy, x, gamma, beta, stats, activation=fctx.activation, want_dx=nx, want_dgamma=ng, want_dbeta=nb)
+            return None, dx, dg if dg is None else dg.to(gamma.dtype), db if db is None else db.to(beta.dtype), None, None, None
+
+    class Linear(torch.autograd.Function):
+        @staticmethod
+        def forward(fctx, lib_ctx, x, w, bias, residual, activation, scale):
+            y, preact = lib_ctx._linear(x, w, bias, residual, activation, scale, ACTIVATIONS[activation] != 0)
+            fctx.save_for_backward(x, w, preact)
+            fctx.lib_ctx, fctx.activation, fctx.scale, fctx.bias_dtype = lib_ctx, activation, scale, None if bias is None else bias.dtype
+            return y
+
+        @staticmethod
+        @once_differentiable
+        def backward(fctx, dy):
+            x, w, preact = fctx.saved_tensors
+            _, nx, nw, nb, nr = fctx.needs_input_grad[:5]
+            dx, dw, db = fctx.lib_ctx.linear_backward(dy, x, w, preact, activation=fctx.activation, scale=fctx.scale, want_dx=nx, want_dw=nw, want_dbias=nb)
+            return None, dx, dw, db if db is None else db.to(fctx.bias_dtype), dy if nr else None, None, None
+
+    _fns = (GroupNorm, Linear)
+    return _fns
+
+
+def _rows(x, lead):
+    """[d0, .., c] with `lead` leading axes kept apart -> (x, stride of the lead axis, row pitch): unit channel stride and ONE stride over the axes
+    between the lead axis and the channels; a copy where x has no such form"""
+    sizes, st = x.shape, x.stride()
+    c = sizes[-1]
+    pitch, span = 0, 1                     # row pitch and rows spanned so far, from the last axis inwards
+    ok = c == 1 or st[-1] == 1
+    for i in range(x.dim() - 2, lead - 1, -1):
+        if sizes[i] != 1:
+            if span == 1:
+                pitch = st[i]
+            elif st[i] != pitch * span:
+                ok = False
+            span *= sizes[i]
+    if ok and (span == 1 or pitch >= c) and (not lead or sizes[0] <= 1 or st[0] >= 0):
+        return x, (st[0] if lead else 0), (c if span == 1 else pitch)
+    x = x.contiguous()
+    return x, span * c, c
 
 
 class Context:
@@ -794,6 +884,186 @@ class Context:
         self._check(self.lib.ttc_upsample_20m(self._h, C.c_void_p(a.data_ptr()), C.c_void_p(b.data_ptr()), T, h, w,
                                               C.c_void_p(out.data_ptr()), self._stream()), "ttc_upsample_20m")
         return out
+
+    # -- channels-last layers ----------------------------------------------------------------
+    def _layer_arg(self, a, what, dtype=None):
+        """numpy -> device; tensors must be on this context's device already"""
+        t = self.torch
+        if a is None:
+            return None
+        if not isinstance(a, t.Tensor):
+            a = self._dev(a)
+        elif not a.is_cuda or a.get_device() != self.device:
+            raise ValueError(f"{what}: a tensor on cuda:{self.device} is needed, got {a.device}")
+        return a if dtype is None or a.dtype == dtype else a.to(dtype)
+
+    def _layer_dtype(self, x, what):
+        t = self.torch
+        code = {t.float32: 0, t.float16: 2, t.bfloat16: 3}.get(x.dtype)
+        if code is None:
+            raise ValueError(f"{what}: float32, float16 or bfloat16, got {x.dtype}")
+        return code
+
+    @staticmethod
+    def _layer_act(activation, what):
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"{what}: unknown activation {activation!r} (one of {', '.join(str(a) for a in ACTIVATIONS)})")
+        return ACTIVATIONS[activation]
+
+    def _layer_ws(self, query, desc, backward, what):
+        nbytes = C.c_size_t(0)
+        st = query(C.byref(desc), backward, C.byref(nbytes))
+        if st != 0:                          # the call itself names the argument
+            return None, 0
+        if not nbytes.value:
+            return None, 0
+        return self.torch.empty(nbytes.value, dtype=self.torch.uint8, device=f"cuda:{self.device}"), nbytes.value
+
+    def _wants_grad(self, what, *tensors):
+        t = self.torch
+        if not t.is_grad_enabled() or not any(isinstance(a, t.Tensor) and a.requires_grad for a in tensors):
+            return False
+        if t.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what}: recording gradients inside a graph capture is not supported (autograd would tie the captured backward pass "
+                               f"to streams outside the graph); call {what} and {what}_backward under torch.no_grad() there")
+        return True
+
+    def group_norm(self, x, gamma=None, beta=None, groups=8, eps=1e-5, activation=None, want_stats=False):
+        """ttc_group_norm: x [n, ..., channels] (cuda fp32 / fp16 / bf16; a channel slice of wider rows is read in place), gamma / beta [channels]
+        -> act(gamma * (x - mean) / sqrt(var + eps) + beta), contiguous, x's type; statistics per sample and group over the axes between.
+        want_stats: also the float32 [n, groups, 2] (mean, 1 / sqrt(var + eps)) that group_norm_backward takes.  Differentiable in x, gamma and
+        beta through torch.autograd (want_stats False)."""
+        x = self._layer_arg(x, "group_norm: x")
+        gamma, beta = (self._layer_arg(a, "group_norm: " + k) for a, k in ((gamma, "gamma"), (beta, "beta")))
+        if self._wants_grad("group_norm", x, gamma, beta):
+            if want_stats:
+                raise ValueError("group_norm: want_stats is for calls without autograd (under torch.no_grad())")
+            return _layer_functions()[0].apply(self, x, gamma, beta, groups, eps, activation)
+        y, stats = self._group_norm(x, gamma, beta, groups, eps, activation, want_stats)
+        return (y, stats) if want_stats else y
+
+    def _norm_desc(self, x, gamma, beta, groups, eps, activation, what):
+        t = self.torch
+        code, act = self._layer_dtype(x, what), self._layer_act(activation, what)
+        if x.dim() < 2:
+            raise ValueError(f"{what}: x must be [n, ..., channels], got {tuple(x.shape)}")
+        n, c = x.shape[0], x.shape[-1]
+        params = []
+        for p, k in ((gamma, "gamma"), (beta, "beta")):
+            if p is not None:
+                if tuple(p.shape) != (c,):
+                    raise ValueError(f"{what}: {k} must be [{c}], got {tuple(p.shape)}")
+                p = p.detach().to(t.float32).contiguous()
+            params.append(p)
+        x, sn, pitch = _rows(x, 1)
+        rows = x.numel() // (n * c) if n and c else 0
+        return x, params[0], params[1], TTCGroupNormDesc(code, act, n, rows, c, int(groups), sn, pitch, float(eps))
+
+    def _group_norm(self, x, gamma, beta, groups, eps, activation, want_stats):
+        t = self.torch
+        x, gamma, beta, d = self._norm_desc(x, gamma, beta, groups, eps, activation, "group_norm")
+        y = t.empty(x.shape, dtype=x.dtype, device=x.device)
+        stats = t.empty((d.n, max(0, d.groups), 2), dtype=t.float32, device=x.device) if want_stats else None
+        if stats is not None and not y.numel():
+            stats.zero_()
+        ws, nb = self._layer_ws(self.lib.ttc_group_norm_workspace, d, 0, "group_norm")
+        ptr = lambda a: None if a is None else a.data_ptr()      # noqa: E731
+        self._check(self.lib.ttc_group_norm(self._h, C.byref(d), ptr(x), ptr(gamma), ptr(beta), ptr(y), ptr(stats), ptr(ws), nb, self._stream()),
+                    "ttc_group_norm")
+        return y, stats
+
+    def group_norm_backward(self, dy, x, gamma, beta, stats, activation=None, want_dx=True, want_dgamma=True, want_dbeta=True):
+        """ttc_group_norm_backward: gradients of group_norm(x, gamma, beta, activation=...) for dy (x's shape and type); `stats` as group_norm(...,
+        want_stats=True) returned them -> (dx, dgamma, dbeta), None where not wanted; dgamma / dbeta float32 [channels]"""
+        t = self.torch
+        what = "group_norm_backward"
+        dy, x, gamma, beta, stats = (self._layer_arg(a, f"{what}: {k}") for a, k in ((dy, "dy"), (x, "x"), (gamma, "gamma"), (beta, "beta"), (stats, "stats")))
+        if stats.dim() != 3 or stats.shape[2] != 2 or stats.shape[0] != x.shape[0] or stats.dtype != t.float32:
+            raise ValueError(f"{what}: stats must be the float32 [{x.shape[0]}, groups, 2] of the forward call, got {stats.dtype} {tuple(stats.shape)}")
+        if dy.shape != x.shape or dy.dtype != x.dtype:
+            raise ValueError(f"{what}: dy must be {x.dtype} {tuple(x.shape)} like x, got {dy.dtype} {tuple(dy.shape)}")
+        x, gamma, beta, d = self._norm_desc(x, gamma, beta, stats.shape[1], 0.0, activation, what)
+        dy, dsn, dpitch = _rows(dy, 1)
+        stats = stats.contiguous()
+        dx = t.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
+        dg, db = (t.empty(d.channels, dtype=t.float32, device=x.device) if w else None for w in (want_dgamma, want_dbeta))
+        ws, nb = self._layer_ws(self.lib.ttc_group_norm_workspace, d, 1, what)
+        ptr = lambda a: None if a is None else a.data_ptr()      # noqa: E731
+        self._check(self.lib.ttc_group_norm_backward(self._h, C.byref(d), ptr(dy), dsn, dpitch, ptr(x), ptr(gamma), ptr(beta), ptr(stats), ptr(dx), ptr(dg),
+                                                     ptr(db), ptr(ws), nb, self._stream()), "ttc_group_norm_backward")
+        return dx, dg, db
+
+    def linear(self, x, w, bias=None, residual=None, activation=None, scale=1.0, want_preact=False):
+        """ttc_linear: residual + scale * act(x w + bias) over the last axis, a 1x1 convolution of channels-last pixels: x [..., cin] (cuda fp32 / fp16 /
+        bf16; a channel slice of wider rows is read in place), w [cin, cout] or the TF kernel [1, 1, cin, cout] in x's type, bias [cout],
+        residual [..., cout] in x's type -> [..., cout], contiguous, x's type.  want_preact: also x w + bias, which linear_backward takes.
+        Differentiable in x, w, bias and residual through torch.autograd (want_preact False)."""
+        x, w, bias, residual = (self._layer_arg(a, "linear: " + k) for a, k in ((x, "x"), (w, "w"), (bias, "bias"), (residual, "residual")))
+        if self._wants_grad("linear", x, w, bias, residual):
+            if want_preact:
+                raise ValueError("linear: want_preact is for calls without autograd (under torch.no_grad())")
+            self._layer_act(activation, "linear")
+            return _layer_functions()[1].apply(self, x, w, bias, residual, activation, scale)
+        y, preact = self._linear(x, w, bias, residual, activation, scale, want_preact)
+        return (y, preact) if want_preact else y
+
+    def _linear_desc(self, x, w, activation, scale, what):
+        code, act = self._layer_dtype(x, what), self._layer_act(activation, what)
+        if w.dim() == 4 and tuple(w.shape[:2]) == (1, 1):
+            w = w[0, 0]
+        if x.dim() < 1 or w.dim() != 2 or w.shape[0] != x.shape[-1] or w.dtype != x.dtype:
+            raise ValueError(f"{what}: x [..., cin] and w [cin, cout] of one type are needed, got {x.dtype} {tuple(x.shape)} and {w.dtype} {tuple(w.shape)}")
+        cin, cout = w.shape
+        if (cout > 1 and w.stride(1) != 1) or (cin > 1 and w.stride(0) < cout):
+            w = w.contiguous()
+        x, _, pitch = _rows(x, 0)
+        rows = x.numel() // cin if cin else 0
+        return x, w, TTCLinearDesc(code, act, rows, cin, cout, pitch, w.stride(0) if cin > 1 else cout, cout, cout, float(scale))
+
+    def _linear(self, x, w, bias, residual, activation, scale, want_preact):
+        t = self.torch
+        x, w, d = self._linear_desc(x, w, activation, scale, "linear")
+        shape = tuple(x.shape[:-1]) + (d.cout,)
+        if bias is not None:
+            if tuple(bias.shape) != (d.cout,):
+                raise ValueError(f"linear: bias must be [{d.cout}], got {tuple(bias.shape)}")
+            bias = bias.detach().to(t.float32).contiguous()
+        if residual is not None:
+            if tuple(residual.shape) != shape or residual.dtype != x.dtype:
+                raise ValueError(f"linear: residual must be {x.dtype} {shape}, got {residual.dtype} {tuple(residual.shape)}")
+            residual, _, d.res_pitch = _rows(residual, 0)
+        y = t.empty(shape, dtype=x.dtype, device=x.device)
+        preact = t.empty(shape, dtype=x.dtype, device=x.device) if want_preact else None
+        ws, nb = self._layer_ws(self.lib.ttc_linear_workspace, d, 0, "linear")
+        ptr = lambda a: None if a is None else a.data_ptr()      # noqa: E731
+        self._check(self.lib.ttc_linear(self._h, C.byref(d), ptr(x), ptr(w), ptr(bias), ptr(residual), ptr(y), ptr(preact), ptr(ws), nb, self._stream()),
+                    "ttc_linear")
+        return y, preact
+
+    def linear_backward(self, dy, x, w, preact=None, activation=None, scale=1.0, want_dx=True, want_dw=True, want_dbias=True):
+        """ttc_linear_backward: gradients of linear(x, w, bias, residual, activation, scale) for dy [..., cout]; `preact` as linear(..., want_preact=True)
+        returned it (needed with an activation) -> (dx, dw, dbias), None where not wanted; dbias float32 [cout].  The residual's gradient is dy."""
+        t = self.torch
+        what = "linear_backward"
+        dy, x, w, preact = (self._layer_arg(a, f"{what}: {k}") for a, k in ((dy, "dy"), (x, "x"), (w, "w"), (preact, "preact")))
+        wshape = w.shape
+        x, w, d = self._linear_desc(x, w, activation, scale, what)
+        shape = tuple(x.shape[:-1]) + (d.cout,)
+        if tuple(dy.shape) != shape or dy.dtype != x.dtype:
+            raise ValueError(f"{what}: dy must be {x.dtype} {shape}, got {dy.dtype} {tuple(dy.shape)}")
+        if d.activation:
+            if preact is None or tuple(preact.shape) != shape or preact.dtype != x.dtype:
+                raise ValueError(f"{what}: activation {activation!r} needs the preact {x.dtype} {shape} of the forward call")
+            preact = preact.contiguous()
+        dy, _, d.dy_pitch = _rows(dy, 0)
+        dx = t.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
+        dw = t.empty(wshape, dtype=x.dtype, device=x.device) if want_dw else None
+        db = t.empty(d.cout, dtype=t.float32, device=x.device) if want_dbias else None
+        ws, nb = self._layer_ws(self.lib.ttc_linear_workspace, d, 1, what)
+        ptr = lambda a: None if a is None else a.data_ptr()      # noqa: E731
+        self._check(self.lib.ttc_linear_backward(self._h, C.byref(d), ptr(dy), ptr(x), ptr(w), ptr(preact), ptr(dx), ptr(dw), ptr(db), ptr(ws), nb,
+                                                 self._stream()), "ttc_linear_backward")
+        return dx, dw, db
 
     # -- debug ----------------------------------------------------------------------------
     def debug_fetch(self, name, shape=None):

@@ -1,0 +1,113 @@
+"""CPU: argument checks of the channels-last layer operators (Context.group_norm / linear) that need no GPU -- the C entries' descriptor checks
+through the workspace queries, and the binding's shape, type and stride rules."""
+import ctypes as C
+
+import pytest
+import torch
+
+from ttc import _lib
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import os
+    if not os.path.exists(_lib.LIB_PATH):
+        import __graft_entry__ as g
+        g.build()
+    return _lib.load()
+
+
+@pytest.fixture
+def host():
+    """a Context without a device: the checks in front of the library calls"""
+    c = object.__new__(_lib.Context)
+    c.torch, c.device, c._h = torch, 0, None
+    return c
+
+
+NORM = dict(dtype=0, activation=0, n=2, rows=9, channels=16, groups=4, x_stride=144, x_pitch=16, eps=1e-5)
+LIN = dict(dtype=0, activation=0, rows=9, cin=16, cout=8, x_pitch=16, w_pitch=8, res_pitch=8, dy_pitch=8, scale=1.0)
+
+
+def _norm(lib, backward=0, **kw):
+    nb = C.c_size_t(123)
+    st = lib.ttc_group_norm_workspace(C.byref(_lib.TTCGroupNormDesc(**{**NORM, **kw})), backward, C.byref(nb))
+    return st, nb.value
+
+
+def _lin(lib, backward=0, **kw):
+    nb = C.c_size_t(123)
+    st = lib.ttc_linear_workspace(C.byref(_lib.TTCLinearDesc(**{**LIN, **kw})), backward, C.byref(nb))
+    return st, nb.value
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=1), dict(dtype=4), dict(activation=-1), dict(activation=6), dict(n=-1), dict(n=65536), dict(rows=-1),
+                                 dict(channels=0), dict(channels=4100, groups=1, x_pitch=4100), dict(groups=0), dict(groups=3), dict(x_pitch=15), dict(x_stride=-1),
+                                 dict(eps=float("nan")), dict(eps=-1.0), dict(eps=float("inf")), dict(rows=1 << 60), dict(x_pitch=1 << 60),
+                                 dict(x_stride=1 << 60)])
+def test_group_norm_descriptor_refusals(lib, bad):
+    assert _norm(lib, **bad) == (1, 0)
+    assert _norm(lib, 1, **bad) == (1, 0)
+
+
+def test_group_norm_descriptor_accepts(lib):
+    for kw in (dict(), dict(rows=1, x_pitch=0), dict(n=1, x_stride=0), dict(channels=4096, groups=4096, x_pitch=4096), dict(eps=0.0), dict(dtype=2), dict(dtype=3)):
+        st, nb = _norm(lib, **kw)
+        assert st == 0 and nb > 0, kw
+    assert _norm(lib, n=0) == (0, 0) and _norm(lib, rows=0) == (0, 0)
+    assert lib.ttc_group_norm_workspace(None, 0, C.byref(C.c_size_t())) == 1
+    assert lib.ttc_group_norm_workspace(C.byref(_lib.TTCGroupNormDesc(**NORM)), 0, None) == 1
+    assert lib.ttc_group_norm(None, C.byref(_lib.TTCGroupNormDesc(**NORM)), None, None, None, None, None, None, 0, None) == 1      # no context
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=1), dict(activation=7), dict(rows=-1), dict(rows=1 << 31), dict(cin=0), dict(cout=0), dict(cin=65537), dict(cout=65537),
+                                 dict(x_pitch=15), dict(w_pitch=7), dict(x_pitch=1 << 31), dict(scale=float("inf")), dict(scale=float("nan")),
+                                 dict(rows=(1 << 31) - 1, cout=65536, w_pitch=65536)])
+def test_linear_descriptor_refusals(lib, bad):
+    assert _lin(lib, **bad) == (1, 0)
+    assert _lin(lib, 1, **bad) == (1, 0)
+
+
+def test_linear_descriptor_accepts(lib):
+    for kw in (dict(), dict(rows=0), dict(rows=1, x_pitch=0), dict(cin=1, w_pitch=0), dict(dtype=3, activation=5)):
+        assert _lin(lib, **kw)[0] == 0, kw
+    assert _lin(lib, 1)[1] > 0 and _lin(lib, 1, rows=0) == (0, 0)
+    assert lib.ttc_linear(None, C.byref(_lib.TTCLinearDesc(**LIN)), None, None, None, None, None, None, None, 0, None) == 1
+
+
+def test_rows_view_rules():
+    """which arrays are read in place, and as what strides"""
+    wide = torch.zeros(3, 5, 7, 24)
+    s = wide[..., 8:24]
+    for x, lead, want in ((s, 1, (5 * 7 * 24, 24)), (s, 0, (0, 24)), (wide[:, 0, :, 4:], 1, (5 * 7 * 24, 24)), (wide[0, 0, 0, :3], 0, (0, 3)),
+                          (wide[:, 1:2, 2:3, :9], 1, (5 * 7 * 24, 9))):
+        y, st, pitch = _lib._rows(x, lead)
+        assert y is x and (st, pitch) == want
+    for x, lead in ((s[:, :, ::2].transpose(1, 2), 1), (s[:, 1:4, 1:5], 1), (wide.transpose(1, 3), 1), (torch.zeros(1, 1, 1, 4).expand(2, 3, 5, 4), 1),
+                    (torch.zeros(2, 3, 1).expand(2, 3, 4), 0)):
+        y, st, pitch = _lib._rows(x, lead)
+        assert y.is_contiguous() and y is not x and pitch == x.shape[-1]
+
+
+def test_binding_refusals(host):
+    x, w = torch.zeros(4, 6, 16), torch.zeros(16, 8)
+    with pytest.raises(ValueError, match="cuda:0"):
+        host.linear(x, w)
+    with pytest.raises(ValueError, match="cuda:0"):
+        host.group_norm(x)
+    with pytest.raises(ValueError, match="unknown activation"):
+        host._linear_desc(x, w, "softmax", 1.0, "linear")
+    for bx, bw in ((x, w.t()), (x, w.half()), (x.double(), w.double()), (x.int(), w.int()), (x, torch.zeros(2, 1, 16, 8)), (torch.zeros(()), w)):
+        with pytest.raises(ValueError, match="linear"):
+            host._linear_desc(bx, bw, None, 1.0, "linear")
+    with pytest.raises(ValueError, match=r"gamma must be \[16\]"):
+        host._norm_desc(x, torch.ones(8), None, 4, 1e-5, None, "group_norm")
+    with pytest.raises(ValueError, match=r"\[n, ..., channels\]"):
+        host._norm_desc(x[0, 0], None, None, 4, 1e-5, None, "group_norm")
+    # TF kernel shape, transposed weight copied, strided weight read in place
+    _, w2, d = host._linear_desc(x, torch.zeros(1, 1, 16, 8), "relu", 0.1, "linear")
+    assert (d.rows, d.cin, d.cout, d.x_pitch, d.w_pitch, d.activation) == (24, 16, 8, 16, 8, 1) and tuple(w2.shape) == (16, 8)
+    _, w2, d = host._linear_desc(x, torch.zeros(16, 20)[:, 3:11], None, 1.0, "linear")
+    assert d.w_pitch == 20
+    _, w2, d = host._linear_desc(x, torch.zeros(8, 16).t(), None, 1.0, "linear")
+    assert d.w_pitch == 8 and w2.is_contiguous()
