@@ -480,15 +480,21 @@ typedef struct {
     int64_t res_pitch, dy_pitch; /* of the residual (ttc_linear) / of dy (ttc_linear_backward)                                    */
     float   scale;               /* y = residual + scale * act(x w + bias): 0.1 in DSen2's residual blocks, else 1                */
 } ttc_linear_desc;
+/* backward: 0 = of ttc_linear, 1 = of ttc_linear_backward without d_preact, TTC_LINEAR_HAVE_PREACT = with it */
+#define TTC_LINEAR_HAVE_PREACT 2
 ttc_status ttc_linear_workspace(const ttc_linear_desc* desc, int32_t backward, size_t* bytes);
-/* d_y [rows, cout]; d_bias [cout] and d_residual [rows, cout] may be NULL; d_preact [rows, cout] (the type of x, may be NULL) receives
+/* 1 where keeping d_preact costs less than forming x w + bias again in the backward pass (never without an activation; not for narrow layers, whose
+ * backward pass reads x anyway) */
+int32_t    ttc_linear_wants_preact(const ttc_linear_desc* desc);
+/* d_y [rows, cout]; d_bias [cout] and d_residual [rows, cout] may be NULL; d_preact [rows, cout] float32 (may be NULL) receives
  * x w + bias for the backward pass. */
 ttc_status ttc_linear(ttc_ctx* ctx, const ttc_linear_desc* desc, const void* d_x, const void* d_w, const float* d_bias, const void* d_residual,
-                      void* d_y, void* d_preact, void* d_ws, size_t ws_bytes, void* stream);
-/* gradients of ttc_linear: with dz = scale * dy * act'(preact), d_dx [rows, cin] = dz w^T, d_dw [cin, cout] = x^T dz (0 for rows = 0),
- * d_dbias [cout] float32 = column sums of dz; each may be NULL.  The residual's gradient is dy.  d_preact: needed with an activation. */
-ttc_status ttc_linear_backward(ttc_ctx* ctx, const ttc_linear_desc* desc, const void* d_dy, const void* d_x, const void* d_w,
-                               const void* d_preact, void* d_dx, void* d_dw, float* d_dbias, void* d_ws, size_t ws_bytes, void* stream);
+                      void* d_y, float* d_preact, void* d_ws, size_t ws_bytes, void* stream);
+/* gradients of ttc_linear: with dz = scale * dy * act'(x w + bias), d_dx [rows, cin] = dz w^T, d_dw [cin, cout] = x^T dz (0 for rows = 0),
+ * d_dbias [cout] float32 = column sums of dz; each may be NULL.  The residual's gradient is dy.  With an activation the argument of act' comes from
+ * d_preact, or, where that is NULL, from x, w and d_bias again (the d_bias of the forward call; not read otherwise). */
+ttc_status ttc_linear_backward(ttc_ctx* ctx, const ttc_linear_desc* desc, const void* d_dy, const void* d_x, const void* d_w, const float* d_bias,
+                               const float* d_preact, void* d_dx, void* d_dw, float* d_dbias, void* d_ws, size_t ws_bytes, void* stream);
 
 /* ---- on-disk formats (host code, no GPU) ----------------------------------------------------------------------------------
  * hkl.load(path) for the numeric arrays of temp/raw (src/download_and_predict_job.py:684-714; written at :462-463, :592-633

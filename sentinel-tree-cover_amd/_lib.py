@@ -26,7 +26,7 @@ EXPORTS = [
     "ttc_border_subtiles", "ttc_seam_adjust", "ttc_reseg_mosaic", "ttc_smooth_strip", "ttc_superresolve_windows", "ttc_count_equal", "ttc_write_geotiff_u8",
     "ttc_predict_tile", "ttc_read_hkl", "ttc_read_hkl_error",
     "ttc_create_v2", "ttc_predict_tile_shaped", "ttc_adjust_shape", "ttc_debug_kernel_flops", "ttc_calibrate_precision",
-    "ttc_group_norm_workspace", "ttc_group_norm", "ttc_group_norm_backward", "ttc_linear_workspace", "ttc_linear", "ttc_linear_backward",
+    "ttc_group_norm_workspace", "ttc_group_norm", "ttc_group_norm_backward", "ttc_linear_workspace", "ttc_linear_wants_preact", "ttc_linear", "ttc_linear_backward",
 ]
 
 # exported for tools/probes and the detector-stage tests, declared in csrc/ttc_internal.h -- not part of the drop-in surface (include/ttc.h)
@@ -178,7 +178,8 @@ def load():
     lib.ttc_group_norm_backward.argtypes = [P, GN, VP, C.c_int64, C.c_int64, VP, VP, VP, VP, VP, VP, VP, VP, SZ, VP]
     lib.ttc_linear_workspace.argtypes = [LN, I32, C.POINTER(SZ)]
     lib.ttc_linear.argtypes = [P, LN, VP, VP, VP, VP, VP, VP, VP, SZ, VP]
-    lib.ttc_linear_backward.argtypes = [P, LN, VP, VP, VP, VP, VP, VP, VP, VP, SZ, VP]
+    lib.ttc_linear_wants_preact.argtypes = [LN]
+    lib.ttc_linear_backward.argtypes = [P, LN, VP, VP, VP, VP, VP, VP, VP, VP, VP, SZ, VP]
     for name in EXPORTS:
         fn = getattr(lib, name)          # AttributeError here == missing export
         if name not in ("ttc_version", "ttc_destroy", "ttc_last_error", "ttc_device_bytes", "ttc_read_hkl_error"):
@@ -278,18 +279,19 @@ def _layer_functions():
     class Linear(torch.autograd.Function):
         @staticmethod
         def forward(fctx, lib_ctx, x, w, bias, residual, activation, scale):
-            y, preact = lib_ctx._linear(x, w, bias, residual, activation, scale, ACTIVATIONS[activation] != 0)
-            fctx.save_for_backward(x, w, preact)
-            fctx.lib_ctx, fctx.activation, fctx.scale, fctx.bias_dtype = lib_ctx, activation, scale, None if bias is None else bias.dtype
+            y, preact = lib_ctx._linear(x, w, bias, residual, activation, scale, True)
+            fctx.save_for_backward(x, w, bias, preact)
+            fctx.lib_ctx, fctx.activation, fctx.scale = lib_ctx, activation, scale
             return y
 
         @staticmethod
         @once_differentiable
         def backward(fctx, dy):
-            x, w, preact = fctx.saved_tensors
+            x, w, bias, preact = fctx.saved_tensors
             _, nx, nw, nb, nr = fctx.needs_input_grad[:5]
-            dx, dw, db = fctx.lib_ctx.linear_backward(dy, x, w, preact, activation=fctx.activation, scale=fctx.scale, want_dx=nx, want_dw=nw, want_dbias=nb)
-            return None, dx, dw, db if db is None else db.to(fctx.bias_dtype), dy if nr else None, None, None
+            dx, dw, db = fctx.lib_ctx.linear_backward(dy, x, w, preact, bias, activation=fctx.activation, scale=fctx.scale, want_dx=nx, want_dw=nw,
+                                                      want_dbias=nb)
+            return None, dx, dw, db if db is None else db.to(bias.dtype), dy if nr else None, None, None
 
     _fns = (GroupNorm, Linear)
     return _fns
@@ -996,7 +998,8 @@ class Context:
     def linear(self, x, w, bias=None, residual=None, activation=None, scale=1.0, want_preact=False):
         """ttc_linear: residual + scale * act(x w + bias) over the last axis, a 1x1 convolution of channels-last pixels: x [..., cin] (cuda fp32 / fp16 /
         bf16; a channel slice of wider rows is read in place), w [cin, cout] or the TF kernel [1, 1, cin, cout] in x's type, bias [cout],
-        residual [..., cout] in x's type -> [..., cout], contiguous, x's type.  want_preact: also x w + bias, which linear_backward takes.
+        residual [..., cout] in x's type -> [..., cout], contiguous, x's type.  want_preact: also what linear_backward takes as `preact`: x w + bias in float32,
+        or None where the backward pass does not need it kept (no activation, or a narrow layer, which forms it again from x).
         Differentiable in x, w, bias and residual through torch.autograd (want_preact False)."""
         x, w, bias, residual = (self._layer_arg(a, "linear: " + k) for a, k in ((x, "x"), (w, "w"), (bias, "bias"), (residual, "residual")))
         if self._wants_grad("linear", x, w, bias, residual):
@@ -1020,48 +1023,54 @@ class Context:
         rows = x.numel() // cin if cin else 0
         return x, w, TTCLinearDesc(code, act, rows, cin, cout, pitch, w.stride(0) if cin > 1 else cout, cout, cout, float(scale))
 
+    def _linear_bias(self, bias, cout, what):
+        if bias is None:
+            return None
+        if tuple(bias.shape) != (cout,):
+            raise ValueError(f"{what}: bias must be [{cout}], got {tuple(bias.shape)}")
+        return bias.detach().to(self.torch.float32).contiguous()
+
     def _linear(self, x, w, bias, residual, activation, scale, want_preact):
         t = self.torch
         x, w, d = self._linear_desc(x, w, activation, scale, "linear")
         shape = tuple(x.shape[:-1]) + (d.cout,)
-        if bias is not None:
-            if tuple(bias.shape) != (d.cout,):
-                raise ValueError(f"linear: bias must be [{d.cout}], got {tuple(bias.shape)}")
-            bias = bias.detach().to(t.float32).contiguous()
+        bias = self._linear_bias(bias, d.cout, "linear")
         if residual is not None:
             if tuple(residual.shape) != shape or residual.dtype != x.dtype:
                 raise ValueError(f"linear: residual must be {x.dtype} {shape}, got {residual.dtype} {tuple(residual.shape)}")
             residual, _, d.res_pitch = _rows(residual, 0)
         y = t.empty(shape, dtype=x.dtype, device=x.device)
-        preact = t.empty(shape, dtype=x.dtype, device=x.device) if want_preact else None
+        preact = t.empty(shape, dtype=t.float32, device=x.device) if want_preact and self.lib.ttc_linear_wants_preact(C.byref(d)) else None
         ws, nb = self._layer_ws(self.lib.ttc_linear_workspace, d, 0, "linear")
         ptr = lambda a: None if a is None else a.data_ptr()      # noqa: E731
         self._check(self.lib.ttc_linear(self._h, C.byref(d), ptr(x), ptr(w), ptr(bias), ptr(residual), ptr(y), ptr(preact), ptr(ws), nb, self._stream()),
                     "ttc_linear")
         return y, preact
 
-    def linear_backward(self, dy, x, w, preact=None, activation=None, scale=1.0, want_dx=True, want_dw=True, want_dbias=True):
-        """ttc_linear_backward: gradients of linear(x, w, bias, residual, activation, scale) for dy [..., cout]; `preact` as linear(..., want_preact=True)
-        returned it (needed with an activation) -> (dx, dw, dbias), None where not wanted; dbias float32 [cout].  The residual's gradient is dy."""
+    def linear_backward(self, dy, x, w, preact=None, bias=None, activation=None, scale=1.0, want_dx=True, want_dw=True, want_dbias=True):
+        """ttc_linear_backward: gradients of linear(x, w, bias, residual, activation, scale) for dy [..., cout] -> (dx, dw, dbias), None where not wanted;
+        dbias float32 [cout].  The residual's gradient is dy.  `preact` as linear(..., want_preact=True) returned it; without it an activation's argument is
+        formed again from x, w and the forward call's bias."""
         t = self.torch
         what = "linear_backward"
-        dy, x, w, preact = (self._layer_arg(a, f"{what}: {k}") for a, k in ((dy, "dy"), (x, "x"), (w, "w"), (preact, "preact")))
+        dy, x, w, preact, bias = (self._layer_arg(a, f"{what}: {k}") for a, k in ((dy, "dy"), (x, "x"), (w, "w"), (preact, "preact"), (bias, "bias")))
         wshape = w.shape
         x, w, d = self._linear_desc(x, w, activation, scale, what)
         shape = tuple(x.shape[:-1]) + (d.cout,)
         if tuple(dy.shape) != shape or dy.dtype != x.dtype:
             raise ValueError(f"{what}: dy must be {x.dtype} {shape}, got {dy.dtype} {tuple(dy.shape)}")
-        if d.activation:
-            if preact is None or tuple(preact.shape) != shape or preact.dtype != x.dtype:
-                raise ValueError(f"{what}: activation {activation!r} needs the preact {x.dtype} {shape} of the forward call")
+        bias = self._linear_bias(bias, d.cout, what)
+        if preact is not None:
+            if tuple(preact.shape) != shape or preact.dtype != t.float32:
+                raise ValueError(f"{what}: preact must be the float32 {shape} of the forward call, got {preact.dtype} {tuple(preact.shape)}")
             preact = preact.contiguous()
         dy, _, d.dy_pitch = _rows(dy, 0)
         dx = t.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
         dw = t.empty(wshape, dtype=x.dtype, device=x.device) if want_dw else None
         db = t.empty(d.cout, dtype=t.float32, device=x.device) if want_dbias else None
-        ws, nb = self._layer_ws(self.lib.ttc_linear_workspace, d, 1, what)
+        ws, nb = self._layer_ws(self.lib.ttc_linear_workspace, d, 1 if preact is None else 2, what)
         ptr = lambda a: None if a is None else a.data_ptr()      # noqa: E731
-        self._check(self.lib.ttc_linear_backward(self._h, C.byref(d), ptr(dy), ptr(x), ptr(w), ptr(preact), ptr(dx), ptr(dw), ptr(db), ptr(ws), nb,
+        self._check(self.lib.ttc_linear_backward(self._h, C.byref(d), ptr(dy), ptr(x), ptr(w), ptr(bias), ptr(preact), ptr(dx), ptr(dw), ptr(db), ptr(ws), nb,
                                                  self._stream()), "ttc_linear_backward")
         return dx, dw, db
 

@@ -34,7 +34,7 @@ struct GemmArgs {
     float alpha;
     // forward epilogue
     int fwd, act;
-    const float* bias; const void* res; long ldr; void* preact;
+    const float* bias; const void* res; long ldr; float* preact;
     int mt, nt;                     // tiles
 };
 
@@ -145,18 +145,6 @@ __device__ __forceinline__ typename Mma<T>::Frag frag(const char* lds, int base,
     }
 }
 
-// what the backward pass reads back: rounded to T, but never across 0 or to infinity (relu's slope is a matter of the sign, and an infinite value
-// would make 0 * inf of the slopes that have long reached their limit)
-template <class T>
-__device__ __forceinline__ float keep_preact(float z) {
-    if constexpr (__is_same(T, f16)) {
-        const float m = fabsf(z);
-        if (m > 65504.0f) return copysignf(65504.0f, z);
-        if (m > 0.0f && m < 5.9604645e-8f) return copysignf(5.9604645e-8f, z);
-    }
-    return z;
-}
-
 // V consecutive columns of one row; `left` of them exist
 template <class T, int V>
 __device__ __forceinline__ void emit(const GemmArgs& a, long row, long col, int left, float (&v)[V]) {
@@ -166,7 +154,6 @@ __device__ __forceinline__ void emit(const GemmArgs& a, long row, long col, int 
         else for (int i = 0; i < left; ++i) p[i] = v[i];
         return;
     }
-    T* out = (T*)a.C + row * a.ldc + col;
     if (!a.fwd) {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] *= a.alpha;
@@ -175,16 +162,14 @@ __device__ __forceinline__ void emit(const GemmArgs& a, long row, long col, int 
 #pragma unroll
             for (int i = 0; i < V; ++i) if (i < left) v[i] += a.bias[col + i];
         }
-        if (a.preact) {
-            T* pp = (T*)a.preact + row * a.ldc + col;
-            float z[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) z[i] = keep_preact<T>(v[i]);
-            if (left >= V) store_vec<T, V>(pp, z);
+        if (a.preact) {                            // in 32 bits: the bias gradient sums slopes taken from it
+            float* pp = a.preact + row * a.ldc + col;
+            if (left >= V) store_vec<float, V>(pp, v);
             else
 #pragma unroll
-                for (int i = 0; i < V; ++i) if (i < left) pp[i] = (T)z[i];
+                for (int i = 0; i < V; ++i) if (i < left) pp[i] = v[i];
         }
+        if (!a.C) return;
         act_vec<V>(v, a.act);
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] *= a.alpha;
@@ -199,6 +184,7 @@ __device__ __forceinline__ void emit(const GemmArgs& a, long row, long col, int 
             for (int i = 0; i < V; ++i) v[i] += r[i];
         }
     }
+    T* out = (T*)a.C + row * a.ldc + col;
     if (left >= V) store_vec<T, V>(out, v);
     else
 #pragma unroll
@@ -286,40 +272,308 @@ __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
     }
 }
 
-// out[i] = alpha * sum of the splits, in split order within 16 interleaved lanes: 64 outputs a block
-template <class T>
-__global__ __launch_bounds__(NT) void k_gemm_reduce(const float* __restrict__ part, int splits, long cnt, float alpha, T* __restrict__ out) {
-    __shared__ float red[16][64];
-    const int e = threadIdx.x & 15, l = threadIdx.x >> 4;
-    const long i0 = (long)blockIdx.x * 64 + e * 4;
+// ---- joining the splits of the contracted index: C = epilogue(sum of the partials), 4 columns a thread, L lanes over the splits -------------------
+// part: [splits][rec] floats, the M x N block first; `tail` further floats of a record (the column sums of dz) go to `tail_out`, times alpha
+template <class T, int L>
+__global__ __launch_bounds__(NT) void k_join(GemmArgs a, const float* __restrict__ part, long rec, int splits, int tail, float* __restrict__ tail_out) {
+    constexpr int E = NT / L;
+    __shared__ float red[L > 1 ? L : 1][E * 4];
+    const int e = threadIdx.x % E, l = threadIdx.x / E;
+    const int nv = (a.N + 3) / 4;
+    const long vecs = a.M * nv, id = (long)blockIdx.x * E + e;
+    long off = 0, row = 0;
+    int col = 0, left = 0;
+    if (id < vecs) { row = id / nv; col = (int)(id % nv) * 4; off = row * a.N + col; left = min(4, a.N - col); }
+    else { col = (int)min((id - vecs) * 4, (long)tail); off = a.M * a.N + col; left = min(4, tail - col); }
     float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (i0 + 4 <= cnt) {
-        for (int k = l; k < splits; k += 16) {
+    if (left == 4) {
+#pragma unroll 4
+        for (int k = l; k < splits; k += L) {
             float v[4];
-            load_vec<float, 4>(part + k * cnt + i0, v);
+            load_vec<float, 4>(part + k * rec + off, v);
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[i] += v[i];
         }
-    } else {
-        for (int k = l; k < splits; k += 16)
+    } else if (left > 0) {
+        for (int k = l; k < splits; k += L)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) if (i0 + i < cnt) s[i] += part[k * cnt + i0 + i];
+            for (int i = 0; i < 4; ++i) if (i < left) s[i] += part[k * rec + off + i];
     }
+    if constexpr (L > 1) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) red[l][e * 4 + i] = s[i];
-    __syncthreads();
-    const long o = (long)blockIdx.x * 64 + threadIdx.x;
-    if (threadIdx.x < 64 && o < cnt) {
-        float t = 0.0f;
-        for (int k = 0; k < 16; ++k) t += red[k][threadIdx.x];
-        out[o] = (T)(t * alpha);
+        for (int i = 0; i < 4; ++i) red[l][e * 4 + i] = s[i];
+        __syncthreads();
+        if (l) return;
+        for (int k = 1; k < L; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] += red[k][e * 4 + i];
+    }
+    if (left <= 0) return;
+    if (id >= vecs) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (i < left) tail_out[col + i] = s[i] * a.alpha;
+    } else if (a.C || a.preact) {
+        emit<T, 4>(a, row, col, left, s);
     }
 }
 
-// ---- dz = scale dy act'(z), and the column sums of dz -----------------------------------------------------------------------------------
+// ---- narrow products: the weights stay in LDS ------------------------------------------------------------------------------------------------
+// x w for cin <= 16-byte steps KS of the contracted index, cout <= 16 FN: bound by the rows' bytes.  A wave takes 16 rows at a time and needs no
+// other wave: x goes from memory straight into fragments (a lane's 16 bytes ARE the fragment), the next rows' while this row's products run, and
+// only the weights sit in LDS, loaded once per workgroup.  16-row steps read KS * FN KB of LDS per KS KB of x: 1/6 of the LDS rate at the memory's.
+template <class T> constexpr int KSTEP = 4 * VE<T>;           // contracted elements of one fragment step: 32 or 16
+
+template <class T, int KS>
+struct RowFrag {
+    uint4 v[KS];
+    __device__ __forceinline__ void load(const T* p, long ld, long row, long rows, int K, int q) {
+        p += row * ld;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) v[s] = load_piece(p + s * KSTEP<T> + q * VE<T>, row < rows ? K - s * KSTEP<T> - q * VE<T> : 0);
+    }
+};
+
+// rows x cols of a weight matrix into an FC image [KP][NP], zero outside
+template <class T, int NP>
+__device__ __forceinline__ void load_image(char* lds, const T* w, long ld, int K, int N, int KP, int tid, int nthreads) {
+    constexpr int PR = NP / VE<T>;
+    for (int id = tid; id < KP * PR; id += nthreads) {
+        const int k = id / PR, f = (id % PR) * VE<T>;
+        *reinterpret_cast<uint4*>(lds + fc_byte<T, NP>(k, f)) = load_piece(w + (long)k * ld + f, k < K ? N - f : 0);
+    }
+}
+
+template <class T, int KS, int FN>
+__global__ __launch_bounds__(NT) void k_narrow(GemmArgs a) {
+    constexpr int NP = FN * 16;
+    constexpr bool PAIR = sizeof(T) == 2 && FN > 1;
+    constexpr int V = PAIR ? 8 : 4, NV = NP / (4 * V);        // columns a lane stores at once, such runs per row
+    __shared__ __attribute__((aligned(16))) char lw[KS * KSTEP<T> * NP * sizeof(T)];
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
+    const long groups = (a.M + 15) / 16, step = (long)gridDim.x * 4;
+    long g = (long)blockIdx.x * 4 + (tid >> 6);
+    RowFrag<T, KS> x;
+    x.load((const T*)a.A, a.lda, g * 16 + r, a.M, (int)a.K, q);
+    load_image<T, NP>(lw, (const T*)a.B, a.ldb, (int)a.K, a.N, KS * KSTEP<T>, tid, NT);
+    __syncthreads();
+    for (; g < groups; g += step) {
+        RowFrag<T, KS> nx;
+        nx.load((const T*)a.A, a.lda, (g + step) * 16 + r, a.M, (int)a.K, q);
+        f32x4 acc[FN];
+#pragma unroll
+        for (int f = 0; f < FN; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int f = 0; f < FN; ++f)
+                acc[f] = Mma<T>::run(frag<T, false, NP, PAIR>(lw, 0, f, s, lane), __builtin_bit_cast(typename Mma<T>::Frag, x.v[s]), acc[f]);
+        const long row = g * 16 + r;
+        if (row < a.M)
+#pragma unroll
+            for (int p = 0; p < NV; ++p) {
+                const int col = p * 4 * V + q * V;
+                if (col >= a.N) continue;
+                float v[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = acc[V == 8 ? 2 * p + i / 4 : p][i & 3];
+                emit<T, V>(a, row, col, a.N - col, v);
+            }
+        x = nx;
+    }
+}
+
+// ---- narrow products: the whole backward pass in one pass over the rows ----------------------------------------------------------------------
+// One wave owns RW rows (the contracted length of one matrix instruction over rows) and does everything for them:
+//   z = x w + b again from the x it reads anyway (cheaper than 4 bytes per output to write and read),  dz = dy act'(z),
+//   dx = dz w^T: a lane's results of the first product are 8 (4) consecutive columns of one row = exactly the operand fragment of this one,
+//   dw += x^T dz: both tiles go through a wave-private piece of LDS and come back transposed; the sums stay in registers for the whole kernel.
+// x and dy are read once, dx written once; per workgroup one record [cin][cout] + column sums of dz leaves for k_join.
+struct NarrowBwd {
+    const void* x; const void* dy; const void* w; const float* bias; const float* z; void* dx; float* part;
+    long M, ldx, ldy, ldw; int K, N, act; float scale;
+    int want_dw, want_db;
+};
+template <class T, int KS, int NS>
+__global__ __launch_bounds__(NT) void k_narrow_bwd(NarrowBwd a) {
+    constexpr int KP = KS * KSTEP<T>, NP = NS * KSTEP<T>, FK = KP / 16, FN = NP / 16;
+    constexpr bool H16 = sizeof(T) == 2;
+    constexpr int RF = H16 ? 2 : 1, RW = 16 * RF, V = VE<T>;
+    typedef typename Mma<T>::Frag Frag;
+    constexpr int TX = RW * KP * sizeof(T), TZ = RW * NP * sizeof(T), IMG = KP * NP * sizeof(T);
+    constexpr int REDB = KP * NP * 4 + NP * 4;
+    constexpr int LDSB = IMG + 4 * (TX + TZ) > REDB ? IMG + 4 * (TX + TZ) : REDB;
+    __shared__ __attribute__((aligned(16))) char lds[LDSB];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
+    char* lw = lds;
+    char* lx = lds + IMG + wave * (TX + TZ);
+    char* lz = lx + TX;
+    const long groups = (a.M + RW - 1) / RW, step = (long)gridDim.x * 4;
+    long g = (long)blockIdx.x * 4 + wave;
+    RowFrag<T, KS> x[RF], nx[RF];
+    RowFrag<T, NS> d[RF], nd[RF];
+#pragma unroll
+    for (int h = 0; h < RF; ++h) {
+        x[h].load((const T*)a.x, a.ldx, g * RW + h * 16 + r, a.M, a.K, q);
+        d[h].load((const T*)a.dy, a.ldy, g * RW + h * 16 + r, a.M, a.N, q);
+    }
+    load_image<T, NP>(lw, (const T*)a.w, a.ldw, a.K, a.N, KP, tid, NT);
+    float bias[NS][V], db[NS][V];
+#pragma unroll
+    for (int p = 0; p < NS; ++p)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int col = p * KSTEP<T> + q * V + i;
+            bias[p][i] = a.bias && col < a.N ? a.bias[col] : 0.0f;
+            db[p][i] = 0.0f;
+        }
+    f32x4 dw[FN][FK];
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FK; ++j) dw[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    __syncthreads();
+    for (; g < groups; g += step) {
+#pragma unroll
+        for (int h = 0; h < RF; ++h) {
+            nx[h].load((const T*)a.x, a.ldx, (g + step) * RW + h * 16 + r, a.M, a.K, q);
+            nd[h].load((const T*)a.dy, a.ldy, (g + step) * RW + h * 16 + r, a.M, a.N, q);
+        }
+#pragma unroll
+        for (int h = 0; h < RF; ++h) {
+            const long row = g * RW + h * 16 + r;
+            Frag dz[NS];
+            if (a.act == TTC_ACT_NONE) {
+#pragma unroll
+                for (int p = 0; p < NS; ++p) {
+                    dz[p] = __builtin_bit_cast(Frag, d[h].v[p]);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) db[p][i] += (float)dz[p][i];
+                }
+            } else {
+                f32x4 z[FN];
+                if (a.z) {
+#pragma unroll
+                    for (int p = 0; p < NS; ++p) {
+                        const int col = p * KSTEP<T> + q * V, left = row < a.M ? a.N - col : 0;
+#pragma unroll
+                        for (int u = 0; u < V / 4; ++u) {
+                            const uint4 t = load_piece(a.z + row * a.N + col + 4 * u, (long)left - 4 * u);
+                            z[p * (V / 4) + u] = __builtin_bit_cast(f32x4, t);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int f = 0; f < FN; ++f) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) z[f][i] = bias[H16 ? f >> 1 : f][H16 ? 4 * (f & 1) + i : i];
+#pragma unroll
+                        for (int s = 0; s < KS; ++s) z[f] = Mma<T>::run(frag<T, false, NP, true>(lw, 0, f, s, lane), __builtin_bit_cast(Frag, x[h].v[s]), z[f]);
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < NS; ++p) {
+                    const Frag dv = __builtin_bit_cast(Frag, d[h].v[p]);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float t = (float)dv[i] * act_slope(z[H16 ? 2 * p + i / 4 : p][i & 3], a.act);
+                        db[p][i] += t;
+                        dz[p][i] = (T)t;                     // operands of the two products have the arrays' type: the one rounding of dz
+                    }
+                }
+            }
+            if (a.dx) {
+                f32x4 o[FK];
+#pragma unroll
+                for (int f = 0; f < FK; ++f) {
+                    o[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int p = 0; p < NS; ++p) {
+                        const uint4 t = *reinterpret_cast<const uint4*>(lw + fc_byte<T, NP>(free_of<T, true>(f, r), p * KSTEP<T> + q * V));
+                        o[f] = Mma<T>::run(__builtin_bit_cast(Frag, t), dz[p], o[f]);
+                    }
+                }
+                if (row < a.M) {
+                    T* out = (T*)a.dx + row * a.K;
+#pragma unroll
+                    for (int p = 0; p < KS; ++p) {
+                        const int col = p * KSTEP<T> + q * V;
+                        float v[V];
+#pragma unroll
+                        for (int i = 0; i < V; ++i) v[i] = o[H16 ? 2 * p + i / 4 : p][i & 3] * a.scale;
+                        if (col + V <= a.K) store_vec<T, V>(out + col, v);
+                        else
+#pragma unroll
+                            for (int i = 0; i < V; ++i) if (col + i < a.K) out[col + i] = (T)v[i];
+                    }
+                }
+            }
+            if (a.want_dw) {
+#pragma unroll
+                for (int s = 0; s < KS; ++s) *reinterpret_cast<uint4*>(lx + fc_byte<T, KP>(h * 16 + r, s * KSTEP<T> + q * V)) = x[h].v[s];
+#pragma unroll
+                for (int p = 0; p < NS; ++p) *reinterpret_cast<uint4*>(lz + fc_byte<T, NP>(h * 16 + r, p * KSTEP<T> + q * V)) = __builtin_bit_cast(uint4, dz[p]);
+            }
+        }
+        if (a.want_dw) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the tiles are this wave's own: LDS serves one wave in order
+            __builtin_amdgcn_wave_barrier();
+            Frag fx[FK];
+#pragma unroll
+            for (int j = 0; j < FK; ++j) fx[j] = frag<T, false, KP, false>(lx, 0, j, 0, lane);
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+                const Frag fz = frag<T, false, NP, false>(lz, 0, i, 0, lane);
+#pragma unroll
+                for (int j = 0; j < FK; ++j) dw[i][j] = Mma<T>::run(fz, fx[j], dw[i][j]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+#pragma unroll
+        for (int h = 0; h < RF; ++h) { x[h] = nx[h]; d[h] = nd[h]; }
+    }
+    if (!a.part) return;
+    // the four waves' sums, in wave order: column sums over the 16 rows of a lane column first
+    float* red = reinterpret_cast<float*>(lds);
+    float* rdb = red + KP * NP;
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1)
+#pragma unroll
+        for (int p = 0; p < NS; ++p)
+#pragma unroll
+            for (int i = 0; i < V; ++i) db[p][i] += __shfl_xor(db[p][i], m);
+    for (int w = 0; w < 4; ++w) {
+        __syncthreads();
+        if (wave != w) continue;
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FK; ++j) {
+                f32x4* c = reinterpret_cast<f32x4*>(red + (16 * j + r) * NP + 16 * i + 4 * q);
+                *c = w ? *c + dw[i][j] : dw[i][j];
+            }
+        if (r == 0)
+#pragma unroll
+            for (int p = 0; p < NS; ++p)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float* c = rdb + p * KSTEP<T> + q * V + i;
+                    *c = w ? *c + db[p][i] : db[p][i];
+                }
+    }
+    __syncthreads();
+    float* out = a.part + (long)blockIdx.x * ((long)a.K * a.N + a.N);
+    for (int i = tid; i < KP * NP; i += NT) {
+        const int k = i / NP, n = i % NP;
+        if (k < a.K && n < a.N) out[k * a.N + n] = red[i];
+    }
+    for (int n = tid; n < a.N; n += NT) out[a.K * a.N + n] = rdb[n];
+}
+
+// ---- wide backward: dz = dy act'(z), and the column sums of dz -----------------------------------------------------------------------------------
 struct DzArgs {
-    const void* dy; const void* z; void* dz; float* part;
-    long rows, dpitch; int N, act; float scale;
+    const void* dy; const float* z; void* dz; float* part;
+    long rows, dpitch; int N, act;
     int cols, rpb; long rows_per;
 };
 template <class T, int V>
@@ -331,19 +585,22 @@ __global__ __launch_bounds__(NT) void k_dz(DzArgs a) {
     float s[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s[i] = 0.0f;
-    if (rl < a.rpb && c0 < a.N)
+    if (rl < a.rpb && c0 < a.N) {
+        const T* dy = (const T*)a.dy + c0;
+#pragma unroll 4
         for (long r = r0 + rl; r < r1; r += a.rpb) {
             float d[V], z[V];
-            load_vec<T, V>((const T*)a.dy + r * a.dpitch + c0, d);
-            if (a.act != TTC_ACT_NONE) load_vec<T, V>((const T*)a.z + r * a.N + c0, z);
+            load_vec<T, V>(dy + r * a.dpitch, d);
+            if (a.act != TTC_ACT_NONE) {
+                load_vec<float, V>(a.z + r * a.N + c0, z);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                d[i] *= a.scale;
-                if (a.act != TTC_ACT_NONE) d[i] *= act_slope(z[i], a.act);
-                s[i] += d[i];
+                for (int i = 0; i < V; ++i) d[i] *= act_slope(z[i], a.act);
             }
-            if (a.dz) store_vec<T, V>((T*)a.dz + r * a.N + c0, d);   // the products take operands of their type: dz is rounded to it once
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[i] += d[i];
+            if (a.dz) store_vec<T, V>((T*)a.dz + r * a.N + c0, d);   // the products take operands of the arrays' type: the one rounding of dz
         }
+    }
     if (!a.part) return;
     if (rl < a.rpb)
 #pragma unroll
@@ -357,19 +614,6 @@ __global__ __launch_bounds__(NT) void k_dz(DzArgs a) {
         a.part[(long)blockIdx.x * a.N + ch] = (float)t;
     }
 }
-// column sums of [rows][N], 16 columns a block
-__global__ __launch_bounds__(NT) void k_col_reduce(const float* __restrict__ part, int rows, int N, float* __restrict__ out) {
-    __shared__ double red[16][17];
-    const int ch = threadIdx.x & 15, l = threadIdx.x >> 4, c = blockIdx.x * 16 + ch;
-    double t = 0.0;
-    if (c < N) for (int r = l; r < rows; r += NT / 16) t += part[(long)r * N + c];
-    red[l][ch] = t;
-    __syncthreads();
-    if (l == 0 && c < N) {
-        for (int i = 1; i < NT / 16; ++i) t += red[i][ch];
-        out[c] = (float)t;
-    }
-}
 template <class T>
 __global__ void k_fill0(T* p, long n) {
     const long i = (long)blockIdx.x * NT + threadIdx.x;
@@ -377,25 +621,75 @@ __global__ void k_fill0(T* p, long n) {
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------------
-template <class T, bool AKC, bool BKC>
-void gemm_launch(GemmArgs a, int splits, hipStream_t s) {
-    a.mt = (int)((a.M + 127) / 128);
-    auto go = [&](auto fn, int bn) {
-        a.nt = (a.N + bn - 1) / bn;
-        hipLaunchKernelGGL(fn, dim3((unsigned)(a.mt * a.nt), splits), dim3(NT), 0, s, a);
-    };
-    // narrower column tiles only where the wide one would be mostly padding
-    if (a.N <= 32) go(k_gemm<T, AKC, BKC, 128, 32, 4>, 32);
-    else if (a.N <= 64) go(k_gemm<T, AKC, BKC, 128, 64, 2>, 64);
-    else go(k_gemm<T, AKC, BKC, 128, 128, 2>, 128);
+int bn_of(long N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }       // column tile: narrower only where the wide one would be mostly padding
+// how many ways the contracted index is split: one where the tiles fill the 256 CUs; else so that about two workgroups per CU run, each with at
+// least `least` of it, and the partials stay under 64 MB
+int gemm_splits(long M, long N, long K, long least) {
+    const long tiles = ((M + 127) / 128) * ((N + bn_of(N) - 1) / bn_of(N));
+    const long fit = std::max<long>(1, (64L << 20) / (M * N * 4));
+    return (int)std::max<long>(1, std::min<long>({512 / tiles, K / least, fit}));
+}
+constexpr long LEAST_K = 128, LEAST_ROWS = 512;
+
+template <class T>
+void join_launch(const GemmArgs& a, const float* part, long rec, int splits, int tail, float* tail_out, hipStream_t s) {
+    const long vecs = a.M * ((a.N + 3) / 4) + (tail + 3) / 4;
+    if (splits > 16) hipLaunchKernelGGL((k_join<T, 16>), dim3((unsigned)((vecs + 15) / 16)), dim3(NT), 0, s, a, part, rec, splits, tail, tail_out);
+    else hipLaunchKernelGGL((k_join<T, 1>), dim3((unsigned)((vecs + NT - 1) / NT)), dim3(NT), 0, s, a, part, rec, splits, tail, tail_out);
 }
 
-// splits of the contracted rows of dw: enough workgroups for two per CU, at least 512 rows each, partials of at most 64 MB
-int dw_splits(const ttc_linear_desc* d) {
-    const long tiles = ((d->cin + 127L) / 128) * ((d->cout + 127L) / 128);
-    const long fit = std::max<long>(1, (64L << 20) / ((long)d->cin * d->cout * 4));
-    return (int)std::max<long>(1, std::min<long>({512 / tiles, d->rows / 512, fit}));
+// C = epilogue(A B) by tiles; ws: splits * M * N floats when splits > 1
+template <class T, bool AKC, bool BKC>
+void gemm_launch(GemmArgs a, int splits, float* ws, hipStream_t s) {
+    GemmArgs j = a;
+    a.k_per = a.K;
+    if (splits > 1) {
+        a.k_per = ((a.K + splits - 1) / splits + BKE<T> - 1) / BKE<T> * BKE<T>;
+        splits = (int)((a.K + a.k_per - 1) / a.k_per);
+    }
+    if (splits > 1) { a.C = ws; a.partial = 1; }
+    a.mt = (int)((a.M + 127) / 128);
+    const int bn = bn_of(a.N);
+    a.nt = (a.N + bn - 1) / bn;
+    auto go = [&](auto fn) { hipLaunchKernelGGL(fn, dim3((unsigned)(a.mt * a.nt), splits), dim3(NT), 0, s, a); };
+    if (bn == 32) go(k_gemm<T, AKC, BKC, 128, 32, 4>);
+    else if (bn == 64) go(k_gemm<T, AKC, BKC, 128, 64, 2>);
+    else go(k_gemm<T, AKC, BKC, 128, 128, 2>);
+    if (splits > 1) join_launch<T>(j, ws, a.M * a.N, splits, 0, nullptr, s);
 }
+
+// the narrow kernels: weights of at most 64 KB as an LDS image whose padded sides are powers of two of 16-byte steps
+int pow2_at_least(int v) { int p = 1; while (p < v) p *= 2; return p; }
+bool narrow_fwd(const ttc_linear_desc* d) {
+    const int step = d->dtype == TTC_DT_F32 ? 16 : 32;
+    return d->cin <= 8 * step && d->cout <= 128;
+}
+bool narrow_bwd(const ttc_linear_desc* d) {
+    if (d->dtype == TTC_DT_F32) return d->cin <= 64 && d->cout <= 64;
+    return d->cin <= 128 && d->cout <= 128 && (d->cin <= 64 || d->cout <= 64);
+}
+template <class T, int KS>
+void narrow_launch_k(const GemmArgs& a, hipStream_t s) {
+    const long groups = (a.M + 15) / 16;
+    const dim3 grid((unsigned)std::min<long>((groups + 3) / 4, 2048));
+    if (a.N <= 16) hipLaunchKernelGGL((k_narrow<T, KS, 1>), grid, dim3(NT), 0, s, a);
+    else if (a.N <= 32) hipLaunchKernelGGL((k_narrow<T, KS, 2>), grid, dim3(NT), 0, s, a);
+    else if (a.N <= 64) hipLaunchKernelGGL((k_narrow<T, KS, 4>), grid, dim3(NT), 0, s, a);
+    else hipLaunchKernelGGL((k_narrow<T, KS, 8>), grid, dim3(NT), 0, s, a);
+}
+template <class T>
+void narrow_launch(const GemmArgs& a, hipStream_t s) {
+    const int ks = (int)((a.K + KSTEP<T> - 1) / KSTEP<T>);
+    if (ks <= 1) narrow_launch_k<T, 1>(a, s);
+    else if (ks <= 2) narrow_launch_k<T, 2>(a, s);
+    else if (ks <= 4) narrow_launch_k<T, 4>(a, s);
+    else narrow_launch_k<T, 8>(a, s);
+}
+int narrow_bwd_blocks(const ttc_linear_desc* d) {
+    const long rw = d->dtype == TTC_DT_F32 ? 64 : 128;        // rows of a workgroup's step
+    return (int)std::min<long>((d->rows + rw - 1) / rw, 512);
+}
+
 int col_vec(int N, int bytes) {
     int v = 16 / bytes;
     while (N % v) v /= 2;
@@ -406,24 +700,39 @@ void dz_geometry(DzArgs& a, int V, int* blocks, int* tiles) {
     a.cols = std::min(cv, NT);
     a.rpb = NT / a.cols;
     *tiles = (cv + a.cols - 1) / a.cols;
-    const long want = std::max<long>(1, 2048 / *tiles), most = std::max<long>(1, a.rows / (4L * a.rpb));
-    long b = std::min(want, most);
+    const long want = std::max<long>(1, 1024 / *tiles), most = std::max<long>(1, a.rows / (4L * a.rpb));
+    const long b = std::min(want, most);
     a.rows_per = std::max<long>(1, (a.rows + b - 1) / b);
     *blocks = (int)((a.rows + a.rows_per - 1) / a.rows_per);
 }
 
-struct BwdWs { size_t dz, sums, dw, total; int blocks; };
-BwdWs linear_ws(const ttc_linear_desc* d) {
+// workspace of the backward pass: z (where it is formed again) | dz | column sums | partial products, each 256-byte aligned
+struct BwdWs { size_t dz, sums, part, total; int blocks, dx_splits, dw_splits; };
+BwdWs linear_ws(const ttc_linear_desc* d, bool have_z) {
     const auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
     BwdWs w{};
+    const size_t cells = (size_t)d->rows * d->cout;
+    if (narrow_bwd(d)) {
+        w.blocks = narrow_bwd_blocks(d);
+        w.total = (size_t)w.blocks * ((size_t)d->cin * d->cout + d->cout) * sizeof(float);
+        return w;
+    }
+    const bool act = d->activation != TTC_ACT_NONE;
     DzArgs z{};
     z.rows = d->rows; z.N = d->cout;
     int tiles;
     dz_geometry(z, col_vec(d->cout, dtype_bytes(d->dtype)), &w.blocks, &tiles);
-    w.sums = d->activation != TTC_ACT_NONE ? up((size_t)d->rows * d->cout * dtype_bytes(d->dtype)) : 0;
-    w.dw = w.sums + up((size_t)w.blocks * d->cout * sizeof(float));
-    const int sp = dw_splits(d);
-    w.total = w.dw + (sp > 1 ? (size_t)sp * d->cin * d->cout * sizeof(float) : 0);
+    w.dz = act && !have_z ? up(cells * sizeof(float)) : 0;
+    w.sums = w.dz + (act ? up(cells * dtype_bytes(d->dtype)) : 0);
+    w.part = w.sums + up((size_t)w.blocks * d->cout * sizeof(float));
+    const size_t zs = act && !have_z ? (size_t)gemm_splits(d->rows, d->cout, d->cin, LEAST_K) : 1;
+    w.dx_splits = gemm_splits(d->rows, d->cin, d->cout, LEAST_K);
+    w.dw_splits = gemm_splits(d->cin, d->cout, d->rows, LEAST_ROWS);
+    size_t part = 0;
+    if (zs > 1) part = zs * cells;
+    if (w.dx_splits > 1) part = std::max(part, (size_t)w.dx_splits * d->rows * d->cin);
+    if (w.dw_splits > 1) part = std::max(part, (size_t)w.dw_splits * d->cin * d->cout);
+    w.total = w.part + part * sizeof(float);
     return w;
 }
 
@@ -441,6 +750,34 @@ const char* linear_check(const ttc_linear_desc* d) {
     if (!std::isfinite(d->scale)) return "scale must be finite";
     return nullptr;
 }
+GemmArgs fwd_args(const ttc_linear_desc* d, const void* x, const void* w) {
+    GemmArgs a{};
+    a.A = x; a.lda = d->x_pitch; a.B = w; a.ldb = d->w_pitch;
+    a.M = d->rows; a.N = d->cout; a.K = d->cin; a.ldc = d->cout;
+    return a;
+}
+
+template <class T>
+void dz_launch(const DzArgs& z, int V, int blocks, int tiles, hipStream_t s) {
+    auto go = [&](auto fn) { hipLaunchKernelGGL(fn, dim3(blocks, tiles), dim3(NT), (size_t)z.rpb * z.cols * V * sizeof(float), s, z); };
+    if (V == 1) go(k_dz<T, 1>);
+    else if (V == 2) go(k_dz<T, 2>);
+    else if (V == 4) go(k_dz<T, 4>);
+    else if constexpr (sizeof(T) == 2) go(k_dz<T, 8>);
+}
+
+template <class T>
+void narrow_bwd_launch(const NarrowBwd& a, int blocks, hipStream_t s) {
+    auto go = [&](auto fn) { hipLaunchKernelGGL(fn, dim3(blocks), dim3(NT), 0, s, a); };
+    if constexpr (sizeof(T) == 4) {
+        if (a.K <= 32) { if (a.N <= 32) go(k_narrow_bwd<T, 2, 2>); else go(k_narrow_bwd<T, 2, 4>); }
+        else { if (a.N <= 32) go(k_narrow_bwd<T, 4, 2>); else go(k_narrow_bwd<T, 4, 4>); }
+    } else {
+        if (a.K > 64) go(k_narrow_bwd<T, 4, 2>);
+        else if (a.N > 64) go(k_narrow_bwd<T, 2, 4>);
+        else go(k_narrow_bwd<T, 2, 2>);
+    }
+}
 
 }  // namespace
 
@@ -450,42 +787,59 @@ ttc_status ttc_linear_workspace(const ttc_linear_desc* d, int32_t backward, size
     if (!bytes) return TTC_ERR_ARG;
     *bytes = 0;
     if (linear_check(d)) return TTC_ERR_ARG;
-    if (backward && d->rows > 0) *bytes = linear_ws(d).total;
+    if (d->rows == 0) return TTC_OK;
+    if (backward) { *bytes = linear_ws(d, backward == TTC_LINEAR_HAVE_PREACT).total; return TTC_OK; }
+    const int sp = narrow_fwd(d) ? 1 : gemm_splits(d->rows, d->cout, d->cin, LEAST_K);
+    if (sp > 1) *bytes = (size_t)sp * d->rows * d->cout * sizeof(float);
     return TTC_OK;
 }
 
+int32_t ttc_linear_wants_preact(const ttc_linear_desc* d) {
+    return !linear_check(d) && d->activation != TTC_ACT_NONE && !narrow_bwd(d);
+}
+
 ttc_status ttc_linear(ttc_ctx* c, const ttc_linear_desc* d, const void* d_x, const void* d_w, const float* d_bias, const void* d_residual,
-                      void* d_y, void* d_preact, void* d_ws, size_t ws_bytes, void* stream) {
-    (void)d_ws; (void)ws_bytes;
+                      void* d_y, float* d_preact, void* d_ws, size_t ws_bytes, void* stream) {
     if (!c) return TTC_ERR_ARG;
     if (const char* e = linear_check(d)) return c->fail(TTC_ERR_ARG, std::string("linear: ") + e);
     if (d_residual && ((d->rows > 1 && d->res_pitch < d->cout) || d->res_pitch > (1L << 30)))
         return c->fail(TTC_ERR_ARG, "linear: res_pitch must be at least cout");
     if (d->rows == 0) return TTC_OK;
-    if (!d_x || !d_w || !d_y) return c->fail(TTC_ERR_ARG, "linear: null pointer");
+    const bool narrow = narrow_fwd(d);
+    const int sp = narrow ? 1 : gemm_splits(d->rows, d->cout, d->cin, LEAST_K);
+    if (!d_x || !d_w || !d_y || (sp > 1 && !d_ws)) return c->fail(TTC_ERR_ARG, "linear: null pointer");
+    if (sp > 1 && ws_bytes < (size_t)sp * d->rows * d->cout * sizeof(float))
+        return c->fail(TTC_ERR_ARG, "linear: workspace smaller than ttc_linear_workspace asks for");
     DeviceGuard dev(c->device);
     if (!dev.ok) return c->fail(TTC_ERR_HIP, "linear: hipSetDevice failed");
-    GemmArgs a{};
-    a.A = d_x; a.lda = d->x_pitch; a.B = d_w; a.ldb = d->w_pitch;
-    a.M = d->rows; a.N = d->cout; a.K = d->cin; a.k_per = d->cin;
-    a.C = d_y; a.ldc = d->cout; a.alpha = d->scale;
+    GemmArgs a = fwd_args(d, d_x, d_w);
+    a.C = d_y; a.alpha = d->scale;
     a.fwd = 1; a.act = d->activation; a.bias = d_bias; a.res = d_residual; a.ldr = d->res_pitch; a.preact = d_preact;
     hipStream_t s = (hipStream_t)stream;
     KTimer t(c, "linear", s);
     const ttc_status st = with_dtype(d->dtype, [&](auto tag) {
-        gemm_launch<decltype(tag), true, false>(a, 1, s);
+        using T = decltype(tag);
+        if (narrow) narrow_launch<T>(a, s);
+        else gemm_launch<T, true, false>(a, sp, (float*)d_ws, s);
         return TTC_OK;
     });
     TTC_HIP(c, hipGetLastError());
     return st;
 }
 
-ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void* d_dy, const void* d_x, const void* d_w, const void* d_preact,
-                               void* d_dx, void* d_dw, float* d_dbias, void* d_ws, size_t ws_bytes, void* stream) {
+ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void* d_dy, const void* d_x, const void* d_w, const float* d_bias,
+                               const float* d_preact, void* d_dx, void* d_dw, float* d_dbias, void* d_ws, size_t ws_bytes, void* stream) {
     if (!c) return TTC_ERR_ARG;
     if (const char* e = linear_check(d)) return c->fail(TTC_ERR_ARG, std::string("linear_backward: ") + e);
     if ((d->rows > 1 && d->dy_pitch < d->cout) || d->dy_pitch > (1L << 30)) return c->fail(TTC_ERR_ARG, "linear_backward: dy_pitch must be at least cout");
     if (!d_dx && !d_dw && !d_dbias) return TTC_OK;
+    const bool act = d->activation != TTC_ACT_NONE, again = act && !d_preact;
+    BwdWs w{};
+    if (d->rows > 0) {
+        w = linear_ws(d, !again);
+        if (!d_dy || ((d_dw || again) && !d_x) || ((d_dx || again) && !d_w) || !d_ws) return c->fail(TTC_ERR_ARG, "linear_backward: null pointer");
+        if (ws_bytes < w.total) return c->fail(TTC_ERR_ARG, "linear_backward: workspace smaller than ttc_linear_workspace asks for");
+    }
     DeviceGuard dev(c->device);
     if (!dev.ok) return c->fail(TTC_ERR_HIP, "linear_backward: hipSetDevice failed");
     hipStream_t s = (hipStream_t)stream;
@@ -498,52 +852,54 @@ ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void*
             if (d_dbias) hipLaunchKernelGGL((k_fill0<float>), dim3((d->cout + NT - 1) / NT), dim3(NT), 0, s, d_dbias, (long)d->cout);
             return TTC_OK;
         }
-        const bool act = d->activation != TTC_ACT_NONE;
-        const BwdWs w = linear_ws(d);
-        if (!d_dy || (d_dw && !d_x) || (d_dx && !d_w) || (act && !d_preact) || (w.total && !d_ws))
-            return c->fail(TTC_ERR_ARG, "linear_backward: null pointer (an activation needs d_preact)");
-        if (ws_bytes < w.total) return c->fail(TTC_ERR_ARG, "linear_backward: workspace smaller than ttc_linear_workspace asks for");
         char* ws = (char*)d_ws;
-        const T* dz = act ? (const T*)ws : (const T*)d_dy;
+        GemmArgs o{};                                        // dw [cin, cout], scaled where the splits are joined
+        o.M = d->cin; o.N = d->cout; o.C = d_dw; o.ldc = d->cout; o.alpha = d->scale;
+        if (narrow_bwd(d)) {
+            NarrowBwd a{};
+            a.x = d_x; a.dy = d_dy; a.w = d_w; a.bias = d_bias; a.z = act ? d_preact : nullptr; a.dx = d_dx;
+            a.part = d_dw || d_dbias ? (float*)ws : nullptr;
+            a.M = d->rows; a.ldx = d->x_pitch; a.ldy = d->dy_pitch; a.ldw = d->w_pitch;
+            a.K = d->cin; a.N = d->cout; a.act = d->activation; a.scale = d->scale; a.want_dw = d_dw != nullptr; a.want_db = d_dbias != nullptr;
+            narrow_bwd_launch<T>(a, w.blocks, s);
+            if (a.part) join_launch<T>(o, a.part, (long)d->cin * d->cout + d->cout, w.blocks, d_dbias ? d->cout : 0, d_dbias, s);
+            return TTC_OK;
+        }
+        const float* z = d_preact;
+        if (again) {                                         // x w + bias in 32 bits
+            GemmArgs a = fwd_args(d, d_x, d_w);
+            GemmArgs zf = a;
+            zf.fwd = 1; zf.act = TTC_ACT_NONE; zf.alpha = 1.0f; zf.bias = d_bias; zf.C = nullptr; zf.preact = (float*)ws;
+            gemm_launch<T, true, false>(zf, gemm_splits(d->rows, d->cout, d->cin, LEAST_K), (float*)(ws + w.part), s);
+            z = (const float*)ws;
+        }
+        const T* dz = act ? (const T*)(ws + w.dz) : (const T*)d_dy;     // without an activation dz is dy itself; the scale is in the epilogues either way
         const long dz_pitch = act ? d->cout : d->dy_pitch;
-        const float alpha = act ? 1.0f : d->scale;           // without an activation dz is dy itself and the scale moves into the epilogues
         if (act || d_dbias) {
-            DzArgs z{};
-            z.dy = d_dy; z.z = d_preact; z.dz = act && (d_dx || d_dw) ? ws : nullptr; z.part = d_dbias ? (float*)(ws + w.sums) : nullptr;
-            z.rows = d->rows; z.dpitch = d->dy_pitch; z.N = d->cout; z.act = d->activation; z.scale = d->scale;
+            DzArgs q{};
+            q.dy = d_dy; q.z = z; q.dz = act && (d_dx || d_dw) ? ws + w.dz : nullptr; q.part = d_dbias ? (float*)(ws + w.sums) : nullptr;
+            q.rows = d->rows; q.dpitch = d->dy_pitch; q.N = d->cout; q.act = d->activation;
             const int V = col_vec(d->cout, sizeof(T));
             int blocks, tiles;
-            dz_geometry(z, V, &blocks, &tiles);
-            auto go = [&](auto fn) { hipLaunchKernelGGL(fn, dim3(blocks, tiles), dim3(NT), (size_t)z.rpb * z.cols * V * sizeof(float), s, z); };
-            if (V == 1) go(k_dz<T, 1>);
-            else if (V == 2) go(k_dz<T, 2>);
-            else if (V == 4) go(k_dz<T, 4>);
-            else if constexpr (sizeof(T) == 2) go(k_dz<T, 8>);
-            if (d_dbias) hipLaunchKernelGGL(k_col_reduce, dim3((d->cout + 15) / 16), dim3(NT), 0, s, z.part, blocks, d->cout, d_dbias);
+            dz_geometry(q, V, &blocks, &tiles);
+            dz_launch<T>(q, V, blocks, tiles, s);
+            if (d_dbias) {
+                GemmArgs b{};
+                b.M = 0; b.N = d->cout; b.alpha = d->scale;
+                join_launch<float>(b, q.part, d->cout, blocks, d->cout, d_dbias, s);
+            }
         }
         if (d_dx) {
             GemmArgs a{};
             a.A = dz; a.lda = dz_pitch; a.B = d_w; a.ldb = d->w_pitch;
-            a.M = d->rows; a.N = d->cin; a.K = d->cout; a.k_per = d->cout;
-            a.C = d_dx; a.ldc = d->cin; a.alpha = alpha;
-            gemm_launch<T, true, true>(a, 1, s);
+            a.M = d->rows; a.N = d->cin; a.K = d->cout;
+            a.C = d_dx; a.ldc = d->cin; a.alpha = d->scale;
+            gemm_launch<T, true, true>(a, w.dx_splits, (float*)(ws + w.part), s);
         }
         if (d_dw) {
-            int sp = dw_splits(d);
-            GemmArgs a{};
-            a.A = d_x; a.lda = d->x_pitch; a.B = dz; a.ldb = dz_pitch;
-            a.M = d->cin; a.N = d->cout; a.K = d->rows;
-            const long step = BKE<T>;
-            a.k_per = ((d->rows + sp - 1) / sp + step - 1) / step * step;
-            sp = (int)((d->rows + a.k_per - 1) / a.k_per);
-            a.C = d_dw; a.ldc = d->cout; a.alpha = alpha;
-            if (sp > 1) { a.C = ws + w.dw; a.partial = 1; }
-            gemm_launch<T, false, false>(a, sp, s);
-            if (sp > 1) {
-                const long n = (long)d->cin * d->cout;
-                hipLaunchKernelGGL((k_gemm_reduce<T>), dim3((unsigned)((n + 63) / 64)), dim3(NT), 0, s, (const float*)(ws + w.dw), sp, n, alpha,
-                                   (T*)d_dw);
-            }
+            GemmArgs a = o;
+            a.A = d_x; a.lda = d->x_pitch; a.B = dz; a.ldb = dz_pitch; a.K = d->rows;
+            gemm_launch<T, false, false>(a, w.dw_splits, (float*)(ws + w.part), s);
         }
         return TTC_OK;
     });

@@ -203,7 +203,9 @@ def check_linear(ctx, x, w, bias, res, act, scale=1.0, dy=None):
     if bias is not None:
         z, S = z + bias.double(), S + bias.double().abs()
     ez = (k + 4) * U * S
-    within("preact", pre.reshape(-1, n), z, ez + h * z.abs() * (1 + h) + 2 * TINY(dt))
+    if pre is not None:
+        assert pre.dtype == torch.float32 and act
+        within("preact", pre.reshape(-1, n), z, ez)
     v, slope = act64(z, act)
     r = res.reshape(-1, n).double() if res is not None else torch.zeros_like(z)
     ref = r + scale * v
@@ -211,12 +213,23 @@ def check_linear(ctx, x, w, bias, res, act, scale=1.0, dy=None):
     within("y", y.reshape(-1, n), ref, e + h * (ref.abs() + e) + TINY(dt))
     if dy is None:
         return y
-    dx, dw, db = ctx.linear_backward(dy, x, w, pre if act else None, activation=act, scale=scale)
+    if act:                                              # the kept argument, or the same formed again: both within the bounds
+        kept = pre if pre is not None else z.float().reshape(y.shape)
+        linear_grads(dy, x, w, bias, act, scale, z, slope, ez, ctx.linear_backward(dy, x, w, kept, activation=act, scale=scale))
+    linear_grads(dy, x, w, bias, act, scale, z, slope, ez, ctx.linear_backward(dy, x, w, None, bias, activation=act, scale=scale))
+    return y
+
+
+def linear_grads(dy, x, w, bias, act, scale, z, slope, ez, got):
+    dt, h = x.dtype, H(x.dtype)
+    k, n = w.shape[-2:]
+    x2, w2 = x.reshape(-1, k).double(), w.reshape(k, n).double()
+    dx, dw, db = got
     assert dx.dtype == dt and dw.dtype == dt and dw.shape == w.shape and db.dtype == torch.float32
     d = dy.reshape(-1, n).double()
     dz = scale * d * slope
-    # the slope comes from the preact (rounded by H, and off by ez before that); relu's is exact but where z is within its error of 0
-    es = 0.8 * (h * (1 + h) + ez + 2 * TINY(dt)) + 64 * U * z.abs().clamp(min=1) * (slope.abs() + U) if act not in (None, "relu") else 0 * z
+    # the slope comes from a preact off by ez; relu's is exact but where z is within its error of 0
+    es = 0.8 * (ez + 2 * U * z.abs()) + 64 * U * z.abs().clamp(min=1) * (slope.abs() + U) if act not in (None, "relu") else 0 * z
     if act == "relu":
         es = (z.abs() <= ez).double()
     edz = abs(scale) * d.abs() * es + 3 * U * dz.abs()
@@ -228,7 +241,6 @@ def check_linear(ctx, x, w, bias, res, act, scale=1.0, dy=None):
     ref = x2.t() @ dz
     e = x2.abs().t() @ rdz + (dz.shape[0] + 8) * U * (x2.abs().t() @ dz.abs())
     within("dw", dw.reshape(k, n), ref, e + h * (ref.abs() + e) + TINY(dt))
-    return y
 
 
 LIN_SHAPES = [  # rows, cin, cout
@@ -286,14 +298,15 @@ def test_linear_hard_values(ctx):
         ok = torch.ones(40, dtype=torch.bool, device="cuda")
         ok[[3, 9]] = False
         assert bool(y[3].isnan().all()) and not bool(y[9].isfinite().any()) and bool(y[ok].isfinite().all())
-    # fp16: a preact past the type's range or below its smallest value keeps its side of 0 and a finite slope
+    # fp16: an argument past the type's range or below its smallest value keeps its side of 0 and a finite slope, kept or formed again
     x = torch.tensor([[300.0], [-300.0], [1e-4], [-1e-4]], device="cuda").half()
     w = torch.tensor([[300.0, 1e-4]], device="cuda").half()
-    y, pre = ctx.linear(x, w, activation="relu", want_preact=True)
-    assert bool(pre.isfinite().all()) and torch.equal(pre > 0, x.expand(4, 2) > 0)
     for act in ("swish", "gelu", "tanh", "sigmoid", "relu"):
-        dx, dw, db = ctx.linear_backward(torch.ones_like(pre), x, w, pre, activation=act)
-        assert bool(dx.isfinite().all()) and bool(dw.isfinite().all()) and bool(db.isfinite().all())
+        for kept in (None, x.float() * w.float()):
+            dx, dw, db = ctx.linear_backward(torch.ones(4, 2, device="cuda").half(), x, w, kept, activation=act)
+            assert bool(dx.isfinite().all()) and bool(dw.isfinite().all()) and bool(db.isfinite().all())
+            if act == "relu":
+                assert torch.equal(db, torch.full_like(db, 2.0))
 
 
 def test_linear_empty(ctx):
@@ -306,13 +319,14 @@ def test_linear_empty(ctx):
 
 
 def test_outputs_not_wanted(ctx):
-    x, w, dy = randn((50, 24), torch.float32, 1), randn((24, 12), torch.float32, 2), randn((50, 12), torch.float32, 3)
-    _, pre = ctx.linear(x, w, activation="tanh", want_preact=True)
-    full = ctx.linear_backward(dy, x, w, pre, activation="tanh")
-    for keep in range(8):
-        got = ctx.linear_backward(dy, x, w, pre, activation="tanh", want_dx=bool(keep & 1), want_dw=bool(keep & 2), want_dbias=bool(keep & 4))
-        for i in range(3):
-            assert (got[i] is None) if not keep >> i & 1 else torch.equal(got[i], full[i])
+    for k, n in ((24, 12), (300, 280)):                  # a narrow layer and a wide one
+        x, w, dy = randn((50, k), torch.float32, 1), randn((k, n), torch.float32, 2), randn((50, n), torch.float32, 3)
+        _, pre = ctx.linear(x, w, activation="tanh", want_preact=True)
+        full = ctx.linear_backward(dy, x, w, pre, activation="tanh")
+        for keep in range(8):
+            got = ctx.linear_backward(dy, x, w, pre, activation="tanh", want_dx=bool(keep & 1), want_dw=bool(keep & 2), want_dbias=bool(keep & 4))
+            for i in range(3):
+                assert (got[i] is None) if not keep >> i & 1 else torch.equal(got[i], full[i])
     xs, g, b = randn((2, 30, 24), torch.float32, 4), randn((24,), torch.float32, 5), randn((24,), torch.float32, 6)
     _, st = ctx.group_norm(xs, g, b, 4, activation="tanh", want_stats=True)
     full = ctx.group_norm_backward(xs, xs, g, b, st, activation="tanh")
@@ -328,7 +342,8 @@ def test_refusals_on_the_device(ctx):
     x, w = torch.zeros(6, 16, device="cuda"), torch.zeros(16, 8, device="cuda")
     for call in (lambda: ctx.linear(x.cpu(), w), lambda: ctx.linear(x, w.half()), lambda: ctx.linear(x, w, bias=torch.zeros(7, device="cuda")),
                  lambda: ctx.linear(x, w, residual=torch.zeros(6, 7, device="cuda")), lambda: ctx.linear(x, w, residual=torch.zeros(6, 8, device="cuda").half()),
-                 lambda: ctx.linear(x, w, activation="softplus"), lambda: ctx.linear_backward(torch.zeros(6, 8, device="cuda"), x, w, None, activation="swish"),
+                 lambda: ctx.linear(x, w, activation="softplus"), lambda: ctx.linear_backward(torch.zeros(6, 8, device="cuda"), x, w, torch.zeros(6, 8, device="cuda").half(), activation="swish"),
+                 lambda: ctx.linear_backward(torch.zeros(6, 8, device="cuda"), x, w, None, torch.zeros(9, device="cuda"), activation="swish"),
                  lambda: ctx.linear_backward(torch.zeros(6, 7, device="cuda"), x, w), lambda: ctx.group_norm(x, torch.ones(8, device="cuda")),
                  lambda: ctx.group_norm_backward(x, x, None, None, torch.zeros(5, 8, 2, device="cuda")),
                  lambda: ctx.group_norm_backward(x.half(), x, None, None, torch.zeros(6, 8, 2, device="cuda"))):
@@ -348,8 +363,8 @@ def test_refusals_on_the_device(ctx):
     assert lib.ttc_group_norm_backward(ctx._h, C.byref(d), p, 96, 16, p, None, None, None, p, None, None, p, 1 << 20, None) == 1
     l = _lib.TTCLinearDesc(0, 2, 6, 16, 8, 16, 8, 8, 8, 1.0)
     assert lib.ttc_linear(ctx._h, C.byref(l), None, p, None, None, p, None, None, 0, None) == 1
-    assert lib.ttc_linear_backward(ctx._h, C.byref(l), p, p, p, None, p, p, None, p, 1 << 20, None) == 1
-    assert lib.ttc_linear_backward(ctx._h, C.byref(l), p, p, p, p, p, p, p, p, 1, None) == 1 and b"workspace" in lib.ttc_last_error(ctx._h)
+    assert lib.ttc_linear_backward(ctx._h, C.byref(l), p, p, None, None, None, p, p, None, p, 1 << 20, None) == 1
+    assert lib.ttc_linear_backward(ctx._h, C.byref(l), p, p, p, None, None, p, p, p, p, 1, None) == 1 and b"workspace" in lib.ttc_last_error(ctx._h)
     torch.cuda.synchronize()
 
 
@@ -360,7 +375,7 @@ def test_two_runs_give_the_same_bits(ctx):
     def once():
         y, pre = ctx.linear(x, w, activation="swish", want_preact=True)
         z, st = ctx.group_norm(xs, g, None, activation="tanh", want_stats=True)
-        return (y, pre) + ctx.linear_backward(dy, x, w, pre, activation="swish") + (z, st) + ctx.group_norm_backward(xs, xs, g, None, st, activation="tanh")
+        return (y,) + ctx.linear_backward(dy, x, w, pre, activation="swish") + (z, st) + ctx.group_norm_backward(xs, xs, g, None, st, activation="tanh")
     a, b = once(), once()
     assert all(torch.equal(u, v) for u, v in zip(a, b))
 
@@ -372,7 +387,7 @@ def _block(ctx, x, p, dy):
     y = ctx.linear(nrm, p["w2"], p["b2"], residual=x, scale=0.1)
     dn, dw2, db2 = ctx.linear_backward(dy, nrm, p["w2"], scale=0.1)
     dh, dg, dbe = ctx.group_norm_backward(dn, h, p["g"], p["be"], st, activation="tanh")
-    dx, dw1, db1 = ctx.linear_backward(dh, x, p["w1"], pre, activation="swish")
+    dx, dw1, db1 = ctx.linear_backward(dh, x, p["w1"], pre, p["b1"], activation="swish")
     return [y, dx + dy, dw1, db1, dg, dbe, dw2, db2]
 
 
