@@ -214,7 +214,7 @@ def _own_product(st):
     y, preact = out if keep else (out, None)
     if not case["train"]:
         return (y,)
-    dx, dw, dbias = ctx.linear_backward(st["dy"], x, w, preact, activation=case["act"], scale=case["scale"], want_dbias=case["bias"])
+    dx, dw, dbias = ctx.linear_backward(st["dy"], x, w, preact, st["bias"], activation=case["act"], scale=case["scale"], want_dbias=case["bias"])
     return (y, dx, dw, dbias) if case["bias"] else (y, dx, dw)
 
 
