@@ -193,8 +193,10 @@ __device__ __forceinline__ void norm_slope(const float (&x)[V], const float (&dy
 #pragma unroll
     for (int i = 0; i < V; ++i) { xh[i] = (x[i] - mean[i]) * rstd[i]; dz[i] = dy[i]; }
     if (act != TTC_ACT_NONE) {
+        float z[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) dz[i] *= act_slope(xh[i] * ga[i] + be[i], act);
+        for (int i = 0; i < V; ++i) z[i] = xh[i] * ga[i] + be[i];
+        slope_vec<V>(dz, z, act);
     }
 }
 

@@ -1,6 +1,7 @@
 // Shared by the channels-last layer operators (group_norm.hip, linear.hip): element types, unaligned vector access, activations.
 #pragma once
 #include <cmath>
+#include <type_traits>
 
 #include "ttc_internal.h"
 
@@ -40,32 +41,68 @@ __device__ __forceinline__ float tanh_rel(float v) {
     return fabsf(v) < 0.5f ? p : e;
 }
 
-__device__ __forceinline__ float act_one(float z, int act) {
+// Normal distribution function of z and e = exp(-z^2 / 2).  cdf(-|z|) = erfc(x) / 2 with x = |z| / sqrt 2, and erfc(x) = exp(-x^2) t P(t),
+// t = 1 / (1 + 0.356 x): P is the degree-9 Chebyshev fit of exp(x^2) erfc(x) / t over t in (0, 1], 2.7e-8 of its value everywhere (0.356 minimises
+// that).  No 1 + erf: the negative tail keeps its relative accuracy.  A quarter of the registers of the library's erfc, which set the kernels' occupancy.
+__device__ __forceinline__ float normal_cdf(float z, float* e) {
+    const float az = fabsf(z), t = __builtin_amdgcn_rcpf(1.0f + (0.356f * 0.70710678f) * az);
+    const float p = 0.20085149f + t * (0.20085289f + t * (0.18806472f + t * (0.16363163f + t * (0.11904900f + t * (0.12201817f
+                    + t * (-0.05494823f + t * (0.17837204f + t * (-0.15755503f + t * 0.03966334f))))))));
+    *e = __expf(-0.5f * z * z);
+    const float h = 0.5f * t * p * *e;
+    return z < 0.0f ? h : 1.0f - h;
+}
+
+// act(z) / act'(z) of one element for a fixed activation
+template <int ACT>
+__device__ __forceinline__ float act_of(float z) {
+    if constexpr (ACT == TTC_ACT_RELU) return z < 0.0f ? 0.0f : z;               // keeps NaN
+    if constexpr (ACT == TTC_ACT_SWISH) return z * sigmoidf(z);
+    if constexpr (ACT == TTC_ACT_SIGMOID) return sigmoidf(z);
+    if constexpr (ACT == TTC_ACT_TANH) return tanh_rel(z);
+    if constexpr (ACT == TTC_ACT_GELU) { float e; return z * normal_cdf(z, &e); }
+    return z;
+}
+// The sigmoid family through e = exp(-|z|), r = 1 / (1 + e): sigmoid(|z|) = r, sigmoid(-|z|) = e r, sigmoid' = e r^2 -- one exponential, one
+// reciprocal, and no 1 - s that cancels for large |z|.
+template <int ACT>
+__device__ __forceinline__ float slope_of(float z) {
+    if constexpr (ACT == TTC_ACT_RELU) return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
+    if constexpr (ACT == TTC_ACT_GELU) { float e; const float c = normal_cdf(z, &e); return c + z * 0.39894228f * e; }
+    if constexpr (ACT == TTC_ACT_SWISH || ACT == TTC_ACT_SIGMOID || ACT == TTC_ACT_TANH) {
+        const float e = __expf((ACT == TTC_ACT_TANH ? -2.0f : -1.0f) * fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e), er2 = e * r * r;
+        if constexpr (ACT == TTC_ACT_SIGMOID) return er2;
+        if constexpr (ACT == TTC_ACT_TANH) return 4.0f * er2;
+        return (z < 0.0f ? e * r : r) + z * er2;
+    }
+    return 1.0f;
+}
+// the same on a vector: ONE uniform branch per vector
+template <class F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
     switch (act) {
-        case TTC_ACT_RELU: return z < 0.0f ? 0.0f : z;               // keeps NaN
-        case TTC_ACT_SWISH: return z * sigmoidf(z);
-        case TTC_ACT_SIGMOID: return sigmoidf(z);
-        case TTC_ACT_TANH: return tanh_rel(z);
-        case TTC_ACT_GELU: return 0.5f * z * erfcf(z * -0.70710678f);   // erfc, not 1 + erf: no cancellation in the negative tail
-        default: return z;
+        case TTC_ACT_RELU: f(std::integral_constant<int, TTC_ACT_RELU>{}); break;
+        case TTC_ACT_SWISH: f(std::integral_constant<int, TTC_ACT_SWISH>{}); break;
+        case TTC_ACT_SIGMOID: f(std::integral_constant<int, TTC_ACT_SIGMOID>{}); break;
+        case TTC_ACT_TANH: f(std::integral_constant<int, TTC_ACT_TANH>{}); break;
+        case TTC_ACT_GELU: f(std::integral_constant<int, TTC_ACT_GELU>{}); break;
+        default: break;
     }
 }
-__device__ __forceinline__ float act_slope(float z, int act) {
-    switch (act) {
-        case TTC_ACT_RELU: return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
-        case TTC_ACT_SWISH: { const float s = sigmoidf(z); return s + z * s * sigmoidf(-z); }
-        case TTC_ACT_SIGMOID: return sigmoidf(z) * sigmoidf(-z);       // not s (1 - s): no cancellation for large z
-        case TTC_ACT_TANH: { const float s = sigmoidf(2.0f * z); return 4.0f * s * sigmoidf(-2.0f * z); }   // 1 - tanh^2, same reason
-        case TTC_ACT_GELU: return 0.5f * erfcf(z * -0.70710678f) + z * 0.39894228f * __expf(-0.5f * z * z);
-        default: return 1.0f;
-    }
-}
-// the same on a vector: one uniform branch per vector
 template <int V>
 __device__ __forceinline__ void act_vec(float (&z)[V], int act) {
-    if (act == TTC_ACT_NONE) return;
+    with_act(act, [&](auto k) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) z[i] = act_one(z[i], act);
+        for (int i = 0; i < V; ++i) z[i] = act_of<decltype(k)::value>(z[i]);
+    });
+}
+// d[i] *= act'(z[i])
+template <int V>
+__device__ __forceinline__ void slope_vec(float (&d)[V], const float (&z)[V], int act) {
+    with_act(act, [&](auto k) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) d[i] *= slope_of<decltype(k)::value>(z[i]);
+    });
 }
 
 template <class F>

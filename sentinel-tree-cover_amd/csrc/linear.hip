@@ -145,50 +145,67 @@ __device__ __forceinline__ typename Mma<T>::Frag frag(const char* lds, int base,
     }
 }
 
-// V consecutive columns of one row; `left` of them exist
+// V consecutive columns of one row, `left` of them exist: the forward epilogue on x w, with the bias and the residual in hand
 template <class T, int V>
-__device__ __forceinline__ void emit(const GemmArgs& a, long row, long col, int left, float (&v)[V]) {
+__device__ __forceinline__ void store_part(T* p, int left, const float (&v)[V]) {
+    if (left >= V) { store_vec<T, V>(p, v); return; }
+#pragma unroll
+    for (int i = 0; i < V; ++i) if (i < left) p[i] = (T)v[i];
+}
+template <class T, int V>
+__device__ __forceinline__ void load_part(const T* p, int left, float (&v)[V]) {
+    if (left >= V) { load_vec<T, V>(p, v); return; }
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = i < left ? (float)p[i] : 0.0f;
+}
+template <class T, int V>
+__device__ __forceinline__ void unpack(const uint4& u, float (&v)[V]) {
+    T t[V];
+    __builtin_memcpy(t, &u, sizeof t);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (float)t[i];
+}
+// Whole cache lines for the stores.  A lane holds pieces of ONE row r = lane & 15 of 16: piece a of columns [0, 4V), piece b of [4V, 8V) by its quarter
+// q = lane >> 4 -- a store of either would write half lines of 16 rows.  Lanes r and r ^ 8 trade pieces: then a lane has columns of ONE half, for rows
+// (r & 7) in a and (r & 7) + 8 in b, and each of the two stores writes 8 whole runs of 8V columns.  (898704 rows, 64 -> 64, bf16: 54.7 -> 45.0 us.)
+__device__ __forceinline__ unsigned ror8(unsigned v) { return __builtin_amdgcn_update_dpp(0u, v, 0x128, 0xf, 0xf, false); }
+template <class R, int V>
+__device__ __forceinline__ void trade(R (&a)[V], R (&b)[V], bool hi) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const unsigned x = __builtin_bit_cast(unsigned, a[i]), y = __builtin_bit_cast(unsigned, b[i]);
+        const unsigned got = ror8(hi ? x : y);
+        a[i] = __builtin_bit_cast(R, hi ? got : x);
+        b[i] = __builtin_bit_cast(R, hi ? y : got);
+    }
+}
+template <class T, int V>
+__device__ __forceinline__ void finish(const GemmArgs& a, long row, int col, int left, float (&v)[V], const float (&bias)[V], const float (&res)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] += bias[i];
+    if (a.preact) store_part<float, V>(a.preact + row * a.ldc + col, left, v);    // in 32 bits: the bias gradient sums slopes taken from it
+    if (!a.C) return;
+    act_vec<V>(v, a.act);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = v[i] * a.alpha + res[i];
+    store_part<T, V>((T*)a.C + row * a.ldc + col, left, v);
+}
+template <class T, int V>
+__device__ __forceinline__ void emit(const GemmArgs& a, long row, int col, int left, float (&v)[V]) {
     if (a.partial) {
-        float* p = (float*)a.C + ((long)blockIdx.y * a.M + row) * a.N + col;
-        if (left >= V) store_vec<float, V>(p, v);
-        else for (int i = 0; i < left; ++i) p[i] = v[i];
-        return;
-    }
-    if (!a.fwd) {
+        store_part<float, V>((float*)a.C + ((long)blockIdx.y * a.M + row) * a.N + col, left, v);
+    } else if (!a.fwd) {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] *= a.alpha;
+        store_part<T, V>((T*)a.C + row * a.ldc + col, left, v);
     } else {
-        if (a.bias) {
+        float bias[V], res[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) if (i < left) v[i] += a.bias[col + i];
-        }
-        if (a.preact) {                            // in 32 bits: the bias gradient sums slopes taken from it
-            float* pp = a.preact + row * a.ldc + col;
-            if (left >= V) store_vec<float, V>(pp, v);
-            else
-#pragma unroll
-                for (int i = 0; i < V; ++i) if (i < left) pp[i] = v[i];
-        }
-        if (!a.C) return;
-        act_vec<V>(v, a.act);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] *= a.alpha;
-        if (a.res) {
-            const T* rp = (const T*)a.res + row * a.ldr + col;
-            float r[V];
-            if (left >= V) load_vec<T, V>(rp, r);
-            else
-#pragma unroll
-                for (int i = 0; i < V; ++i) r[i] = i < left ? (float)rp[i] : 0.0f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] += r[i];
-        }
+        for (int i = 0; i < V; ++i) bias[i] = res[i] = 0.0f;
+        if (a.bias) load_part<float, V>(a.bias + col, left, bias);
+        if (a.res) load_part<T, V>((const T*)a.res + row * a.ldr + col, left, res);
+        finish<T, V>(a, row, col, left, v, bias, res);
     }
-    T* out = (T*)a.C + row * a.ldc + col;
-    if (left >= V) store_vec<T, V>(out, v);
-    else
-#pragma unroll
-        for (int i = 0; i < V; ++i) if (i < left) out[i] = (T)v[i];
 }
 
 // ---- the tile kernel --------------------------------------------------------------------------------------------------------------------
@@ -245,28 +262,28 @@ __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
         }
         __syncthreads();
     }
-    const int r = lane & 15, q = lane >> 4;
+    const int r = lane & 15, q = lane >> 4, hi = r >> 3;
+    constexpr int V = VE<T>, NV = WN / (4 * V);               // columns a lane stores at once, such runs of a wave
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-        const long row = m0 + wm * WM + j * 16 + r;
-        if (row >= a.M) continue;
-        if constexpr (sizeof(T) == 2) {
+        const long base = m0 + wm * WM + j * 16;
 #pragma unroll
-            for (int p = 0; p < FN / 2; ++p) {
-                const int col = n0 + wn * WN + 32 * p + 8 * q;
-                if (col >= a.N) continue;
-                float v[8];
+        for (int p = 0; p < NV; p += 2) {
+            float v[2][V];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { v[i] = acc[2 * p][j][i]; v[4 + i] = acc[2 * p + 1][j][i]; }
-                emit<T, 8>(a, row, col, a.N - col, v);
-            }
-        } else {
+            for (int u = 0; u < 2; ++u)
+                if (p + u < NV)
 #pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                const int col = n0 + wn * WN + 16 * i + 4 * q;
-                if (col >= a.N) continue;
-                float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                emit<T, 4>(a, row, col, a.N - col, v);
+                    for (int i = 0; i < V; ++i) v[u][i] = acc[V == 8 ? 2 * (p + u) + i / 4 : p + u][j][i & 3];
+            if (p + 1 < NV) trade(v[0], v[1], hi);
+            const int col = n0 + wn * WN + (p + (p + 1 < NV ? hi : 0)) * 4 * V + q * V;
+            if (col >= a.N) continue;
+            if (p + 1 < NV) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if (base + (r & 7) + 8 * u < a.M) emit<T, V>(a, base + (r & 7) + 8 * u, col, a.N - col, v[u]);
+            } else if (base + r < a.M) {
+                emit<T, V>(a, base + r, col, a.N - col, v[0]);
             }
         }
     }
@@ -323,13 +340,61 @@ __global__ __launch_bounds__(NT) void k_join(GemmArgs a, const float* __restrict
 // only the weights sit in LDS, loaded once per workgroup.  16-row steps read KS * FN KB of LDS per KS KB of x: 1/6 of the LDS rate at the memory's.
 template <class T> constexpr int KSTEP = 4 * VE<T>;           // contracted elements of one fragment step: 32 or 16
 
-template <class T, int KS>
+// drop the first `n` elements of 16 bytes (all of them for n >= VE), zeros come in
+template <class T>
+__device__ __forceinline__ uint4 drop_front(uint4 v, int n) {
+    const int bits = n * 8 * (int)sizeof(T);
+    unsigned long lo = v.x | (unsigned long)v.y << 32, hi = v.z | (unsigned long)v.w << 32;
+    if (bits >= 64) { lo = hi; hi = 0; }
+    const int b = bits & 63;
+    if (b) { lo = lo >> b | hi << (64 - b); hi >>= b; }
+    if (bits >= 128) lo = 0;
+    return make_uint4((unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32));
+}
+
+// 16 rows of an array: the wave's row 0 is a scalar base, a lane's place in them a 32-bit byte offset that never changes (the narrow kernels take pitches
+// up to 2^24 elements).  Rows past the last read the last row: nothing of them is stored or summed.
+struct Rows16 {
+    const char* p;
+    long pitch;                     // bytes
+    long rows;
+    __device__ __forceinline__ const char* base(long r0) const { return p + min(r0, rows - 1) * pitch; }
+    __device__ __forceinline__ unsigned row(long r0, int r) const {      // of row r0 + r, from base(r0)
+        const long left = rows - 1 - min(r0, rows - 1);
+        return (unsigned)(left >= 15 ? r : min(r, (int)left)) * (unsigned)pitch;
+    }
+};
+template <class T>
+__device__ __forceinline__ Rows16 rows16(const void* p, long pitch, long rows) { return {(const char*)p, pitch * (long)sizeof(T), rows}; }
+
+// One row's fragment pieces (zero past K).  A piece that sticks out of the row is read so that it ENDS with the row and shifted down: no lane takes an
+// element-by-element path (rows shorter than 16 bytes apart).
+// FULL: K is exactly the fragment's width.
+template <class T, int KS, bool FULL>
 struct RowFrag {
     uint4 v[KS];
-    __device__ __forceinline__ void load(const T* p, long ld, long row, long rows, int K, int q) {
-        p += row * ld;
+    __device__ __forceinline__ void load(const Rows16& a, long r0, int r, int K, int q) {
+        const char* p = a.base(r0);
+        const unsigned o = a.row(r0, r);
+        if (FULL || K == KS * KSTEP<T>) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) v[s] = load_piece(p + s * KSTEP<T> + q * VE<T>, row < rows ? K - s * KSTEP<T> - q * VE<T> : 0);
+            for (int s = 0; s < KS; ++s) __builtin_memcpy(&v[s], p + (o + q * 16u) + s * 64, 16);
+        } else if (K >= VE<T>) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) __builtin_memcpy(&v[s], p + (o + (unsigned)min(s * KSTEP<T> + q * VE<T>, K - VE<T>) * (unsigned)sizeof(T)), 16);
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) v[s] = load_piece((const T*)(p + o), s || q ? 0 : K);
+        }
+    }
+    // after the load has arrived (kept apart from it so that the next rows' loads stay in flight)
+    __device__ __forceinline__ void trim(int K, int q) {
+        if (FULL || K == KS * KSTEP<T> || K < VE<T>) return;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int c = s * KSTEP<T> + q * VE<T>;
+            v[s] = drop_front<T>(v[s], c - min(c, K - VE<T>));
+        }
     }
 };
 
@@ -343,22 +408,53 @@ __device__ __forceinline__ void load_image(char* lds, const T* w, long ld, int K
     }
 }
 
-template <class T, int KS, int FN>
+// FULL: cout is exactly 16 FN and no preact leaves: no lane sits out but in the last rows.  A kernel of its own, because the ragged epilogue's
+// addresses and masks cost 50 registers (898704 rows, 64 -> 64 with residual, bf16: 165 registers, 3 waves per SIMD, 77 us against 122, 4 and 65 us).
+template <class T, int KS, int FN, bool FULL>
 __global__ __launch_bounds__(NT) void k_narrow(GemmArgs a) {
     constexpr int NP = FN * 16;
     constexpr bool PAIR = sizeof(T) == 2 && FN > 1;
     constexpr int V = PAIR ? 8 : 4, NV = NP / (4 * V);        // columns a lane stores at once, such runs per row
     __shared__ __attribute__((aligned(16))) char lw[KS * KSTEP<T> * NP * sizeof(T)];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), K = (int)a.K;
     const long groups = (a.M + 15) / 16, step = (long)gridDim.x * 4;
-    long g = (long)blockIdx.x * 4 + (tid >> 6);
-    RowFrag<T, KS> x;
-    x.load((const T*)a.A, a.lda, g * 16 + r, a.M, (int)a.K, q);
-    load_image<T, NP>(lw, (const T*)a.B, a.ldb, (int)a.K, a.N, KS * KSTEP<T>, tid, NT);
+    long g = (long)blockIdx.x * 4 + wave;
+    constexpr int NG = NV == 1 ? 1 : NV / 2, NR = NV == 1 ? 1 : 2;        // column runs of a lane after the trade, rows of each
+    const int hi = NV == 1 ? 0 : r >> 3, r0 = NV == 1 ? r : r & 7;
+    const int c0 = hi * 4 * V + q * V;                        // first column of a lane's run p: NR * p * 4 V further
+    const Rows16 ax = rows16<T>(a.A, a.lda, a.M), ar = rows16<T>(a.res, a.ldr, a.M);
+    RowFrag<T, KS, false> x0, x1;
+    uint4 res0[NG][NR], res1[NG][NR];                         // V elements of the residual each
+    auto load_res = [&](uint4 (&to)[NG][NR], long row) {
+        const char* p = ar.base(row);
+#pragma unroll
+        for (int u = 0; u < NR; ++u) {
+            const unsigned o = ar.row(row, r0 + 8 * u) + c0 * (unsigned)sizeof(T);
+#pragma unroll
+            for (int i = 0; i < NG; ++i) __builtin_memcpy(&to[i][u], p + o + i * NR * 4 * V * (int)sizeof(T), V * sizeof(T));
+        }
+    };
+    x0.load(ax, g * 16, r, K, q);
+    if (FULL && a.res) load_res(res0, g * 16);
+    load_image<T, NP>(lw, (const T*)a.B, a.ldb, K, a.N, KS * KSTEP<T>, tid, NT);
+    float bias[NG][V];
+#pragma unroll
+    for (int p = 0; p < NG; ++p)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int col = NR * p * 4 * V + c0 + i;
+            bias[p][i] = a.bias && col < a.N ? a.bias[col] : 0.0f;
+        }
     __syncthreads();
-    for (; g < groups; g += step) {
-        RowFrag<T, KS> nx;
-        nx.load((const T*)a.A, a.lda, (g + step) * 16 + r, a.M, (int)a.K, q);
+    // two register sets in turn: a copy between them would wait for the loads it is there to overlap
+    auto rows = [&](RowFrag<T, KS, false>& x, uint4 (&res)[NG][NR], RowFrag<T, KS, false>& nx, uint4 (&nres)[NG][NR]) {
+        const long base = g * 16;
+        nx.load(ax, base + step * 16, r, K, q);
+        if (FULL && a.res) load_res(nres, base + step * 16);
+        x.trim(K, q);
+        int here = 0;
+        asm volatile("" : "+v"(here));        // the weights are read from LDS for every 16 rows: kept in registers they cost a wave per SIMD (fp32 64 -> 64: 144 -> 135 us)
         f32x4 acc[FN];
 #pragma unroll
         for (int f = 0; f < FN; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -366,19 +462,52 @@ __global__ __launch_bounds__(NT) void k_narrow(GemmArgs a) {
         for (int s = 0; s < KS; ++s)
 #pragma unroll
             for (int f = 0; f < FN; ++f)
-                acc[f] = Mma<T>::run(frag<T, false, NP, PAIR>(lw, 0, f, s, lane), __builtin_bit_cast(typename Mma<T>::Frag, x.v[s]), acc[f]);
-        const long row = g * 16 + r;
-        if (row < a.M)
+                acc[f] = Mma<T>::run(frag<T, false, NP, PAIR>(lw + here, 0, f, s, lane), __builtin_bit_cast(typename Mma<T>::Frag, x.v[s]), acc[f]);
+        const int left = (int)min(a.M - base, 16L);
 #pragma unroll
-            for (int p = 0; p < NV; ++p) {
-                const int col = p * 4 * V + q * V;
-                if (col >= a.N) continue;
-                float v[V];
+        for (int p = 0; p < NG; ++p) {
+            float v[NR][V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[i] = acc[V == 8 ? 2 * p + i / 4 : p][i & 3];
-                emit<T, V>(a, row, col, a.N - col, v);
+            for (int u = 0; u < NR; ++u)
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[u][i] = acc[V == 8 ? 2 * (NR * p + u) + i / 4 : NR * p + u][i & 3];
+            if constexpr (NR == 2) trade(v[0], v[1], hi);
+            const int col = NR * p * 4 * V + c0;
+#pragma unroll
+            for (int u = 0; u < NR; ++u) {
+                if constexpr (FULL) {
+                    if (r0 + 8 * u >= left) continue;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[u][i] += bias[p][i];
+                    act_vec<V>(v[u], a.act);
+                    if (a.res) {
+                        float rv[V];
+                        unpack<T, V>(res[p][u], rv);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) v[u][i] = v[u][i] * a.alpha + rv[i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) v[u][i] *= a.alpha;
+                    }
+                    store_vec<T, V>((T*)((char*)a.C + base * NP * (long)sizeof(T) + (unsigned)(((r0 + 8 * u) * NP + col) * (int)sizeof(T))), v[u]);
+                    continue;
+                }
+                const long row = base + r0 + 8 * u;
+                if (r0 + 8 * u >= left || col >= a.N) continue;
+                float rv[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) rv[i] = 0.0f;
+                if (a.res) load_part<T, V>((const T*)a.res + row * a.ldr + col, a.N - col, rv);
+                finish<T, V>(a, row, col, a.N - col, v[u], bias[p], rv);
             }
-        x = nx;
+        }
+        g += step;
+    };
+    for (;;) {
+        if (g >= groups) break;
+        rows(x0, res0, x1, res1);
+        if (g >= groups) break;
+        rows(x1, res1, x0, res0);
     }
 }
 
@@ -393,8 +522,9 @@ struct NarrowBwd {
     long M, ldx, ldy, ldw; int K, N, act; float scale;
     int want_dw, want_db;
 };
-template <class T, int KS, int NS>
-__global__ __launch_bounds__(NT) void k_narrow_bwd(NarrowBwd a) {
+// FULL: cin and cout are exactly the padded sides and the preact is formed again (as in k_narrow: no masks, no second set of addresses).
+template <class T, int KS, int NS, bool FULL>
+__global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) void k_narrow_bwd(NarrowBwd a) {
     constexpr int KP = KS * KSTEP<T>, NP = NS * KSTEP<T>, FK = KP / 16, FN = NP / 16;
     constexpr bool H16 = sizeof(T) == 2;
     constexpr int RF = H16 ? 2 : 1, RW = 16 * RF, V = VE<T>;
@@ -403,18 +533,19 @@ __global__ __launch_bounds__(NT) void k_narrow_bwd(NarrowBwd a) {
     constexpr int REDB = KP * NP * 4 + NP * 4;
     constexpr int LDSB = IMG + 4 * (TX + TZ) > REDB ? IMG + 4 * (TX + TZ) : REDB;
     __shared__ __attribute__((aligned(16))) char lds[LDSB];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, q = lane >> 4;
+    const Rows16 ax = rows16<T>(a.x, a.ldx, a.M), ad = rows16<T>(a.dy, a.ldy, a.M);
     char* lw = lds;
     char* lx = lds + IMG + wave * (TX + TZ);
     char* lz = lx + TX;
     const long groups = (a.M + RW - 1) / RW, step = (long)gridDim.x * 4;
     long g = (long)blockIdx.x * 4 + wave;
-    RowFrag<T, KS> x[RF], nx[RF];
-    RowFrag<T, NS> d[RF], nd[RF];
+    RowFrag<T, KS, FULL> x0[RF], x1[RF];
+    RowFrag<T, NS, FULL> d0[RF], d1[RF];
 #pragma unroll
     for (int h = 0; h < RF; ++h) {
-        x[h].load((const T*)a.x, a.ldx, g * RW + h * 16 + r, a.M, a.K, q);
-        d[h].load((const T*)a.dy, a.ldy, g * RW + h * 16 + r, a.M, a.N, q);
+        x0[h].load(ax, g * RW + h * 16, r, a.K, q);
+        d0[h].load(ad, g * RW + h * 16, r, a.N, q);
     }
     load_image<T, NP>(lw, (const T*)a.w, a.ldw, a.K, a.N, KP, tid, NT);
     float bias[NS][V], db[NS][V];
@@ -432,15 +563,22 @@ __global__ __launch_bounds__(NT) void k_narrow_bwd(NarrowBwd a) {
 #pragma unroll
         for (int j = 0; j < FK; ++j) dw[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     __syncthreads();
-    for (; g < groups; g += step) {
+    // two register sets in turn: a copy between them would wait for the loads it is there to overlap
+    auto rows = [&](RowFrag<T, KS, FULL> (&x)[RF], RowFrag<T, NS, FULL> (&d)[RF], RowFrag<T, KS, FULL> (&nx)[RF], RowFrag<T, NS, FULL> (&nd)[RF]) {
 #pragma unroll
         for (int h = 0; h < RF; ++h) {
-            nx[h].load((const T*)a.x, a.ldx, (g + step) * RW + h * 16 + r, a.M, a.K, q);
-            nd[h].load((const T*)a.dy, a.ldy, (g + step) * RW + h * 16 + r, a.M, a.N, q);
+            nx[h].load(ax, (g + step) * RW + h * 16, r, a.K, q);
+            nd[h].load(ad, (g + step) * RW + h * 16, r, a.N, q);
         }
 #pragma unroll
         for (int h = 0; h < RF; ++h) {
             const long row = g * RW + h * 16 + r;
+            x[h].trim(a.K, q);
+            d[h].trim(a.N, q);
+            const int left = (int)max(min(a.M - (g * RW + h * 16), 16L), 0L);
+            if (r >= left)
+#pragma unroll
+                for (int p = 0; p < NS; ++p) d[h].v[p] = make_uint4(0, 0, 0, 0);
             Frag dz[NS];
             if (a.act == TTC_ACT_NONE) {
 #pragma unroll
@@ -451,13 +589,13 @@ __global__ __launch_bounds__(NT) void k_narrow_bwd(NarrowBwd a) {
                 }
             } else {
                 f32x4 z[FN];
-                if (a.z) {
+                if (!FULL && a.z) {
 #pragma unroll
                     for (int p = 0; p < NS; ++p) {
-                        const int col = p * KSTEP<T> + q * V, left = row < a.M ? a.N - col : 0;
+                        const int col = p * KSTEP<T> + q * V, cols = r < left ? a.N - col : 0;
 #pragma unroll
                         for (int u = 0; u < V / 4; ++u) {
-                            const uint4 t = load_piece(a.z + row * a.N + col + 4 * u, (long)left - 4 * u);
+                            const uint4 t = load_piece(a.z + row * a.N + col + 4 * u, (long)cols - 4 * u);
                             z[p * (V / 4) + u] = __builtin_bit_cast(f32x4, t);
                         }
                     }
@@ -473,11 +611,14 @@ __global__ __launch_bounds__(NT) void k_narrow_bwd(NarrowBwd a) {
 #pragma unroll
                 for (int p = 0; p < NS; ++p) {
                     const Frag dv = __builtin_bit_cast(Frag, d[h].v[p]);
+                    float t[V], zz[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) { t[i] = (float)dv[i]; zz[i] = z[H16 ? 2 * p + i / 4 : p][i & 3]; }
+                    slope_vec<V>(t, zz, a.act);
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        const float t = (float)dv[i] * act_slope(z[H16 ? 2 * p + i / 4 : p][i & 3], a.act);
-                        db[p][i] += t;
-                        dz[p][i] = (T)t;                     // operands of the two products have the arrays' type: the one rounding of dz
+                        db[p][i] += t[i];
+                        dz[p][i] = (T)t[i];                  // operands of the two products have the arrays' type: the one rounding of dz
                     }
                 }
             }
@@ -492,18 +633,34 @@ __global__ __launch_bounds__(NT) void k_narrow_bwd(NarrowBwd a) {
                         o[f] = Mma<T>::run(__builtin_bit_cast(Frag, t), dz[p], o[f]);
                     }
                 }
-                if (row < a.M) {
-                    T* out = (T*)a.dx + row * a.K;
+                const int hi = KS == 1 ? 0 : r >> 3;
 #pragma unroll
-                    for (int p = 0; p < KS; ++p) {
-                        const int col = p * KSTEP<T> + q * V;
-                        float v[V];
+                for (int p = 0; p < KS; p += 2) {
+                    unsigned v[2][4];
 #pragma unroll
-                        for (int i = 0; i < V; ++i) v[i] = o[H16 ? 2 * p + i / 4 : p][i & 3] * a.scale;
-                        if (col + V <= a.K) store_vec<T, V>(out + col, v);
-                        else
+                    for (int u = 0; u < (KS == 1 ? 1 : 2); ++u) {
+                        T t[V];
 #pragma unroll
-                            for (int i = 0; i < V; ++i) if (col + i < a.K) out[col + i] = (T)v[i];
+                        for (int i = 0; i < V; ++i) t[i] = (T)(o[H16 ? 2 * (p + u) + i / 4 : p + u][i & 3] * a.scale);
+                        __builtin_memcpy(v[u], t, 16);
+                    }
+                    if constexpr (KS > 1) trade(v[0], v[1], hi);
+                    const int col = (p + hi) * KSTEP<T> + q * V;
+#pragma unroll
+                    for (int u = 0; u < (KS == 1 ? 1 : 2); ++u) {
+                        const int rr = KS == 1 ? r : (r & 7) + 8 * u;
+                        if (rr >= left) continue;
+                        if constexpr (FULL) {
+                            __builtin_memcpy((char*)a.dx + (g * RW + h * 16) * KP * (long)sizeof(T) + (unsigned)((rr * KP + col) * (int)sizeof(T)), v[u], 16);
+                            continue;
+                        }
+                        if (col >= a.K) continue;
+                        T* out = (T*)a.dx + (g * RW + h * 16 + rr) * a.K + col;
+                        if (col + V <= a.K) { __builtin_memcpy(out, v[u], 16); continue; }
+                        T t[V];
+                        __builtin_memcpy(t, v[u], 16);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) if (col + i < a.K) out[i] = t[i];
                     }
                 }
             }
@@ -529,8 +686,13 @@ __global__ __launch_bounds__(NT) void k_narrow_bwd(NarrowBwd a) {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
-#pragma unroll
-        for (int h = 0; h < RF; ++h) { x[h] = nx[h]; d[h] = nd[h]; }
+        g += step;
+    };
+    for (;;) {
+        if (g >= groups) break;
+        rows(x0, d0, x1, d1);
+        if (g >= groups) break;
+        rows(x1, d1, x0, d0);
     }
     if (!a.part) return;
     // the four waves' sums, in wave order: column sums over the 16 rows of a lane column first
@@ -593,8 +755,7 @@ __global__ __launch_bounds__(NT) void k_dz(DzArgs a) {
             load_vec<T, V>(dy + r * a.dpitch, d);
             if (a.act != TTC_ACT_NONE) {
                 load_vec<float, V>(a.z + r * a.N + c0, z);
-#pragma unroll
-                for (int i = 0; i < V; ++i) d[i] *= act_slope(z[i], a.act);
+                slope_vec<V>(d, z, a.act);
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) s[i] += d[i];
@@ -660,11 +821,14 @@ void gemm_launch(GemmArgs a, int splits, float* ws, hipStream_t s) {
 
 // the narrow kernels: weights of at most 64 KB as an LDS image whose padded sides are powers of two of 16-byte steps
 int pow2_at_least(int v) { int p = 1; while (p < v) p *= 2; return p; }
+constexpr long NARROW_PITCH = 1L << 24;                       // 15 rows of them fit a 32-bit byte offset
 bool narrow_fwd(const ttc_linear_desc* d) {
+    if (d->x_pitch > NARROW_PITCH || d->res_pitch > NARROW_PITCH) return false;
     const int step = d->dtype == TTC_DT_F32 ? 16 : 32;
     return d->cin <= 8 * step && d->cout <= 128;
 }
 bool narrow_bwd(const ttc_linear_desc* d) {
+    if (d->x_pitch > NARROW_PITCH || d->dy_pitch > NARROW_PITCH) return false;
     if (d->dtype == TTC_DT_F32) return d->cin <= 64 && d->cout <= 64;
     return d->cin <= 128 && d->cout <= 128 && (d->cin <= 64 || d->cout <= 64);
 }
@@ -672,10 +836,15 @@ template <class T, int KS>
 void narrow_launch_k(const GemmArgs& a, hipStream_t s) {
     const long groups = (a.M + 15) / 16;
     const dim3 grid((unsigned)std::min<long>((groups + 3) / 4, 2048));
-    if (a.N <= 16) hipLaunchKernelGGL((k_narrow<T, KS, 1>), grid, dim3(NT), 0, s, a);
-    else if (a.N <= 32) hipLaunchKernelGGL((k_narrow<T, KS, 2>), grid, dim3(NT), 0, s, a);
-    else if (a.N <= 64) hipLaunchKernelGGL((k_narrow<T, KS, 4>), grid, dim3(NT), 0, s, a);
-    else hipLaunchKernelGGL((k_narrow<T, KS, 8>), grid, dim3(NT), 0, s, a);
+    auto go = [&](auto fn) {
+        constexpr int FN = decltype(fn)::value;
+        if (a.N == FN * 16 && !a.preact) hipLaunchKernelGGL((k_narrow<T, KS, FN, true>), grid, dim3(NT), 0, s, a);
+        else hipLaunchKernelGGL((k_narrow<T, KS, FN, false>), grid, dim3(NT), 0, s, a);
+    };
+    if (a.N <= 16) go(std::integral_constant<int, 1>{});
+    else if (a.N <= 32) go(std::integral_constant<int, 2>{});
+    else if (a.N <= 64) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 8>{});
 }
 template <class T>
 void narrow_launch(const GemmArgs& a, hipStream_t s) {
@@ -768,15 +937,18 @@ void dz_launch(const DzArgs& z, int V, int blocks, int tiles, hipStream_t s) {
 
 template <class T>
 void narrow_bwd_launch(const NarrowBwd& a, int blocks, hipStream_t s) {
-    auto go = [&](auto fn) { hipLaunchKernelGGL(fn, dim3(blocks), dim3(NT), 0, s, a); };
-    if constexpr (sizeof(T) == 4) {
-        if (a.K <= 32) { if (a.N <= 32) go(k_narrow_bwd<T, 2, 2>); else go(k_narrow_bwd<T, 2, 4>); }
-        else { if (a.N <= 32) go(k_narrow_bwd<T, 4, 2>); else go(k_narrow_bwd<T, 4, 4>); }
-    } else {
-        if (a.K > 64) go(k_narrow_bwd<T, 4, 2>);
-        else if (a.N > 64) go(k_narrow_bwd<T, 2, 4>);
-        else go(k_narrow_bwd<T, 2, 2>);
-    }
+    auto go = [&](auto ks, auto ns) {
+        constexpr int KS = decltype(ks)::value, NS = decltype(ns)::value;
+        if (a.K == KS * KSTEP<T> && a.N == NS * KSTEP<T> && !a.z) hipLaunchKernelGGL((k_narrow_bwd<T, KS, NS, true>), dim3(blocks), dim3(NT), 0, s, a);
+        else hipLaunchKernelGGL((k_narrow_bwd<T, KS, NS, false>), dim3(blocks), dim3(NT), 0, s, a);
+    };
+    constexpr std::integral_constant<int, 2> two{};
+    constexpr std::integral_constant<int, 4> four{};
+    const int half = 2 * KSTEP<T>;
+    if (a.K <= half && a.N <= half) go(two, two);
+    else if (a.K <= half) go(two, four);
+    else if (a.N <= half) go(four, two);
+    else if constexpr (sizeof(T) == 4) go(four, four);
 }
 
 }  // namespace
