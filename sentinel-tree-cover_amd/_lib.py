@@ -888,16 +888,17 @@ class Context:
         return out
 
     # -- channels-last layers ----------------------------------------------------------------
-    def _layer_arg(self, a, what, dtype=None):
+    # A call's checks, strides, descriptor and scratch size follow from its shapes, strides, types and options alone: they are worked out once per such
+    # combination (a "plan") and looked up afterwards -- a small layer's call is bound by this host code.
+    def _layer_arg(self, a, what):
         """numpy -> device; tensors must be on this context's device already"""
-        t = self.torch
         if a is None:
             return None
-        if not isinstance(a, t.Tensor):
-            a = self._dev(a)
-        elif not a.is_cuda or a.get_device() != self.device:
+        if not isinstance(a, self.torch.Tensor):
+            return self._dev(a)
+        if a.get_device() != self.device:
             raise ValueError(f"{what}: a tensor on cuda:{self.device} is needed, got {a.device}")
-        return a if dtype is None or a.dtype == dtype else a.to(dtype)
+        return a
 
     def _layer_dtype(self, x, what):
         t = self.torch
@@ -912,18 +913,34 @@ class Context:
             raise ValueError(f"{what}: unknown activation {activation!r} (one of {', '.join(str(a) for a in ACTIVATIONS)})")
         return ACTIVATIONS[activation]
 
-    def _layer_ws(self, query, desc, backward, what):
+    def _layer_vec(self, p, c, what):
+        """a per-channel parameter as contiguous float32"""
+        if p is None:
+            return None
+        if p.dim() != 1 or p.shape[0] != c:
+            raise ValueError(f"{what} must be [{c}], got {tuple(p.shape)}")
+        return p if p.dtype is self.torch.float32 and p.is_contiguous() else p.detach().to(self.torch.float32).contiguous()
+
+    def _layer_plan(self, key, make):
+        plans = self.__dict__.setdefault("_plans", {})
+        plan = plans.get(key)
+        if plan is None:
+            if len(plans) >= 4096:           # shapes that never come back must not pile up
+                plans.clear()
+            plan = plans[key] = make()
+        return plan
+
+    def _layer_ws(self, query, desc, backward):
+        """scratch bytes of a call; 0 where the descriptor is refused: the call itself names the argument"""
         nbytes = C.c_size_t(0)
-        st = query(C.byref(desc), backward, C.byref(nbytes))
-        if st != 0:                          # the call itself names the argument
-            return None, 0
-        if not nbytes.value:
-            return None, 0
-        return self.torch.empty(nbytes.value, dtype=self.torch.uint8, device=f"cuda:{self.device}"), nbytes.value
+        return nbytes.value if query(C.byref(desc), backward, C.byref(nbytes)) == 0 else 0
+
+    def _layer_stream(self):
+        return self.torch._C._cuda_getCurrentRawStream(self.device)
 
     def _wants_grad(self, what, *tensors):
         t = self.torch
-        if not t.is_grad_enabled() or not any(isinstance(a, t.Tensor) and a.requires_grad for a in tensors):
+        if not t.is_grad_enabled() or not any(a is not None and a.requires_grad for a in tensors):
             return False
         if t.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{what}: recording gradients inside a graph capture is not supported (autograd would tie the captured backward pass "
@@ -935,8 +952,7 @@ class Context:
         -> act(gamma * (x - mean) / sqrt(var + eps) + beta), contiguous, x's type; statistics per sample and group over the axes between.
         want_stats: also the float32 [n, groups, 2] (mean, 1 / sqrt(var + eps)) that group_norm_backward takes.  Differentiable in x, gamma and
         beta through torch.autograd (want_stats False)."""
-        x = self._layer_arg(x, "group_norm: x")
-        gamma, beta = (self._layer_arg(a, "group_norm: " + k) for a, k in ((gamma, "gamma"), (beta, "beta")))
+        x, gamma, beta = self._layer_arg(x, "group_norm: x"), self._layer_arg(gamma, "group_norm: gamma"), self._layer_arg(beta, "group_norm: beta")
         if self._wants_grad("group_norm", x, gamma, beta):
             if want_stats:
                 raise ValueError("group_norm: want_stats is for calls without autograd (under torch.no_grad())")
@@ -944,34 +960,34 @@ class Context:
         y, stats = self._group_norm(x, gamma, beta, groups, eps, activation, want_stats)
         return (y, stats) if want_stats else y
 
-    def _norm_desc(self, x, gamma, beta, groups, eps, activation, what):
-        t = self.torch
+    def _norm_plan(self, x, groups, eps, activation, what, backward):
+        """-> (descriptor, its reference, copy x first, scratch bytes, channels)"""
         code, act = self._layer_dtype(x, what), self._layer_act(activation, what)
         if x.dim() < 2:
             raise ValueError(f"{what}: x must be [n, ..., channels], got {tuple(x.shape)}")
         n, c = x.shape[0], x.shape[-1]
-        params = []
-        for p, k in ((gamma, "gamma"), (beta, "beta")):
-            if p is not None:
-                if tuple(p.shape) != (c,):
-                    raise ValueError(f"{what}: {k} must be [{c}], got {tuple(p.shape)}")
-                p = p.detach().to(t.float32).contiguous()
-            params.append(p)
-        x, sn, pitch = _rows(x, 1)
+        v, sn, pitch = _rows(x, 1)
         rows = x.numel() // (n * c) if n and c else 0
-        return x, params[0], params[1], TTCGroupNormDesc(code, act, n, rows, c, int(groups), sn, pitch, float(eps))
+        d = TTCGroupNormDesc(code, act, n, rows, c, int(groups), sn, pitch, float(eps))
+        return d, C.byref(d), v is not x, self._layer_ws(self.lib.ttc_group_norm_workspace, d, backward), c
 
     def _group_norm(self, x, gamma, beta, groups, eps, activation, want_stats):
         t = self.torch
-        x, gamma, beta, d = self._norm_desc(x, gamma, beta, groups, eps, activation, "group_norm")
-        y = t.empty(x.shape, dtype=x.dtype, device=x.device)
-        stats = t.empty((d.n, max(0, d.groups), 2), dtype=t.float32, device=x.device) if want_stats else None
-        if stats is not None and not y.numel():
-            stats.zero_()
-        ws, nb = self._layer_ws(self.lib.ttc_group_norm_workspace, d, 0, "group_norm")
-        ptr = lambda a: None if a is None else a.data_ptr()      # noqa: E731
-        self._check(self.lib.ttc_group_norm(self._h, C.byref(d), ptr(x), ptr(gamma), ptr(beta), ptr(y), ptr(stats), ptr(ws), nb, self._stream()),
-                    "ttc_group_norm")
+        d, ref, copy, nb, c = self._layer_plan(("norm", x.shape, x.stride(), x.dtype, groups, eps, activation),
+                                               lambda: self._norm_plan(x, groups, eps, activation, "group_norm", 0))
+        gamma, beta = self._layer_vec(gamma, c, "group_norm: gamma"), self._layer_vec(beta, c, "group_norm: beta")
+        if copy:
+            x = x.contiguous()
+        y = x.new_empty(x.shape)
+        stats = None
+        if want_stats:
+            stats = x.new_empty((d.n, max(0, d.groups), 2), dtype=t.float32)
+            if not y.numel():
+                stats.zero_()
+        ws = x.new_empty(nb, dtype=t.uint8) if nb else None
+        self._check(self.lib.ttc_group_norm(self._h, ref, x.data_ptr(), gamma.data_ptr() if gamma is not None else None,
+                                            beta.data_ptr() if beta is not None else None, y.data_ptr(), stats.data_ptr() if want_stats else None,
+                                            ws.data_ptr() if nb else None, nb, self._layer_stream()), "ttc_group_norm")
         return y, stats
 
     def group_norm_backward(self, dy, x, gamma, beta, stats, activation=None, want_dx=True, want_dgamma=True, want_dbeta=True):
@@ -984,15 +1000,25 @@ class Context:
             raise ValueError(f"{what}: stats must be the float32 [{x.shape[0]}, groups, 2] of the forward call, got {stats.dtype} {tuple(stats.shape)}")
         if dy.shape != x.shape or dy.dtype != x.dtype:
             raise ValueError(f"{what}: dy must be {x.dtype} {tuple(x.shape)} like x, got {dy.dtype} {tuple(dy.shape)}")
-        x, gamma, beta, d = self._norm_desc(x, gamma, beta, stats.shape[1], 0.0, activation, what)
-        dy, dsn, dpitch = _rows(dy, 1)
+        groups = stats.shape[1]
+
+        def make():
+            v, dsn, dpitch = _rows(dy, 1)
+            return self._norm_plan(x, groups, 0.0, activation, what, 1) + (v is not dy, dsn, dpitch)
+        d, ref, copy, nb, c, dcopy, dsn, dpitch = self._layer_plan(("norm_bwd", x.shape, x.stride(), dy.stride(), x.dtype, groups, activation), make)
+        gamma, beta = self._layer_vec(gamma, c, what + ": gamma"), self._layer_vec(beta, c, what + ": beta")
+        if copy:
+            x = x.contiguous()
+        if dcopy:
+            dy = dy.contiguous()
         stats = stats.contiguous()
-        dx = t.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
-        dg, db = (t.empty(d.channels, dtype=t.float32, device=x.device) if w else None for w in (want_dgamma, want_dbeta))
-        ws, nb = self._layer_ws(self.lib.ttc_group_norm_workspace, d, 1, what)
+        dx = x.new_empty(x.shape) if want_dx else None
+        dg = x.new_empty(c, dtype=t.float32) if want_dgamma else None
+        db = x.new_empty(c, dtype=t.float32) if want_dbeta else None
+        ws = x.new_empty(nb, dtype=t.uint8) if nb else None
         ptr = lambda a: None if a is None else a.data_ptr()      # noqa: E731
-        self._check(self.lib.ttc_group_norm_backward(self._h, C.byref(d), ptr(dy), dsn, dpitch, ptr(x), ptr(gamma), ptr(beta), ptr(stats), ptr(dx), ptr(dg),
-                                                     ptr(db), ptr(ws), nb, self._stream()), "ttc_group_norm_backward")
+        self._check(self.lib.ttc_group_norm_backward(self._h, ref, dy.data_ptr(), dsn, dpitch, x.data_ptr(), ptr(gamma), ptr(beta), stats.data_ptr(), ptr(dx),
+                                                     ptr(dg), ptr(db), ptr(ws), nb, self._layer_stream()), "ttc_group_norm_backward")
         return dx, dg, db
 
     def linear(self, x, w, bias=None, residual=None, activation=None, scale=1.0, want_preact=False):
@@ -1001,7 +1027,8 @@ class Context:
         residual [..., cout] in x's type -> [..., cout], contiguous, x's type.  want_preact: also what linear_backward takes as `preact`: x w + bias in float32,
         or None where the backward pass does not need it kept (no activation, or a narrow layer, which forms it again from x).
         Differentiable in x, w, bias and residual through torch.autograd (want_preact False)."""
-        x, w, bias, residual = (self._layer_arg(a, "linear: " + k) for a, k in ((x, "x"), (w, "w"), (bias, "bias"), (residual, "residual")))
+        x, w, bias, residual = (self._layer_arg(x, "linear: x"), self._layer_arg(w, "linear: w"), self._layer_arg(bias, "linear: bias"),
+                                self._layer_arg(residual, "linear: residual"))
         if self._wants_grad("linear", x, w, bias, residual):
             if want_preact:
                 raise ValueError("linear: want_preact is for calls without autograd (under torch.no_grad())")
@@ -1011,40 +1038,47 @@ class Context:
         return (y, preact) if want_preact else y
 
     def _linear_desc(self, x, w, activation, scale, what):
+        """-> (descriptor, copy x first, copy w first, shape of y)"""
         code, act = self._layer_dtype(x, what), self._layer_act(activation, what)
         if w.dim() == 4 and tuple(w.shape[:2]) == (1, 1):
             w = w[0, 0]
         if x.dim() < 1 or w.dim() != 2 or w.shape[0] != x.shape[-1] or w.dtype != x.dtype:
             raise ValueError(f"{what}: x [..., cin] and w [cin, cout] of one type are needed, got {x.dtype} {tuple(x.shape)} and {w.dtype} {tuple(w.shape)}")
         cin, cout = w.shape
-        if (cout > 1 and w.stride(1) != 1) or (cin > 1 and w.stride(0) < cout):
-            w = w.contiguous()
-        x, _, pitch = _rows(x, 0)
+        wcopy = (cout > 1 and w.stride(1) != 1) or (cin > 1 and w.stride(0) < cout)
+        v, _, pitch = _rows(x, 0)
         rows = x.numel() // cin if cin else 0
-        return x, w, TTCLinearDesc(code, act, rows, cin, cout, pitch, w.stride(0) if cin > 1 else cout, cout, cout, float(scale))
-
-    def _linear_bias(self, bias, cout, what):
-        if bias is None:
-            return None
-        if tuple(bias.shape) != (cout,):
-            raise ValueError(f"{what}: bias must be [{cout}], got {tuple(bias.shape)}")
-        return bias.detach().to(self.torch.float32).contiguous()
+        d = TTCLinearDesc(code, act, rows, cin, cout, pitch, cout if wcopy or cin <= 1 else w.stride(0), cout, cout, float(scale))
+        return d, v is not x, wcopy, tuple(x.shape[:-1]) + (cout,)
 
     def _linear(self, x, w, bias, residual, activation, scale, want_preact):
         t = self.torch
-        x, w, d = self._linear_desc(x, w, activation, scale, "linear")
-        shape = tuple(x.shape[:-1]) + (d.cout,)
-        bias = self._linear_bias(bias, d.cout, "linear")
-        if residual is not None:
-            if tuple(residual.shape) != shape or residual.dtype != x.dtype:
-                raise ValueError(f"linear: residual must be {x.dtype} {shape}, got {residual.dtype} {tuple(residual.shape)}")
-            residual, _, d.res_pitch = _rows(residual, 0)
-        y = t.empty(shape, dtype=x.dtype, device=x.device)
-        preact = t.empty(shape, dtype=t.float32, device=x.device) if want_preact and self.lib.ttc_linear_wants_preact(C.byref(d)) else None
-        ws, nb = self._layer_ws(self.lib.ttc_linear_workspace, d, 0, "linear")
-        ptr = lambda a: None if a is None else a.data_ptr()      # noqa: E731
-        self._check(self.lib.ttc_linear(self._h, C.byref(d), ptr(x), ptr(w), ptr(bias), ptr(residual), ptr(y), ptr(preact), ptr(ws), nb, self._stream()),
-                    "ttc_linear")
+
+        def make():
+            d, copy, wcopy, shape = self._linear_desc(x, w, activation, scale, "linear")
+            rcopy = False
+            if residual is not None:
+                if tuple(residual.shape) != shape or residual.dtype != x.dtype:
+                    raise ValueError(f"linear: residual must be {x.dtype} {shape}, got {residual.dtype} {tuple(residual.shape)}")
+                v, _, d.res_pitch = _rows(residual, 0)
+                rcopy = v is not residual
+            return d, C.byref(d), copy, wcopy, rcopy, shape, self._layer_ws(self.lib.ttc_linear_workspace, d, 0), self.lib.ttc_linear_wants_preact(C.byref(d))
+        res_key = None if residual is None else (residual.shape, residual.stride(), residual.dtype)
+        d, ref, copy, wcopy, rcopy, shape, nb, keeps = self._layer_plan(
+            ("linear", x.shape, x.stride(), x.dtype, w.shape, w.stride(), w.dtype, activation, scale, res_key), make)
+        bias = self._layer_vec(bias, d.cout, "linear: bias")
+        if copy:
+            x = x.contiguous()
+        if wcopy:
+            w = w.contiguous()
+        if rcopy:
+            residual = residual.contiguous()
+        y = x.new_empty(shape)
+        preact = x.new_empty(shape, dtype=t.float32) if want_preact and keeps else None
+        ws = x.new_empty(nb, dtype=t.uint8) if nb else None
+        self._check(self.lib.ttc_linear(self._h, ref, x.data_ptr(), w.data_ptr(), bias.data_ptr() if bias is not None else None,
+                                        residual.data_ptr() if residual is not None else None, y.data_ptr(), preact.data_ptr() if preact is not None else None,
+                                        ws.data_ptr() if nb else None, nb, self._layer_stream()), "ttc_linear")
         return y, preact
 
     def linear_backward(self, dy, x, w, preact=None, bias=None, activation=None, scale=1.0, want_dx=True, want_dw=True, want_dbias=True):
@@ -1054,24 +1088,35 @@ class Context:
         t = self.torch
         what = "linear_backward"
         dy, x, w, preact, bias = (self._layer_arg(a, f"{what}: {k}") for a, k in ((dy, "dy"), (x, "x"), (w, "w"), (preact, "preact"), (bias, "bias")))
-        wshape = w.shape
-        x, w, d = self._linear_desc(x, w, activation, scale, what)
-        shape = tuple(x.shape[:-1]) + (d.cout,)
-        if tuple(dy.shape) != shape or dy.dtype != x.dtype:
-            raise ValueError(f"{what}: dy must be {x.dtype} {shape}, got {dy.dtype} {tuple(dy.shape)}")
-        bias = self._linear_bias(bias, d.cout, what)
-        if preact is not None:
-            if tuple(preact.shape) != shape or preact.dtype != t.float32:
+
+        def make():
+            d, copy, wcopy, shape = self._linear_desc(x, w, activation, scale, what)
+            if tuple(dy.shape) != shape or dy.dtype != x.dtype:
+                raise ValueError(f"{what}: dy must be {x.dtype} {shape}, got {dy.dtype} {tuple(dy.shape)}")
+            if preact is not None and (tuple(preact.shape) != shape or preact.dtype != t.float32):
                 raise ValueError(f"{what}: preact must be the float32 {shape} of the forward call, got {preact.dtype} {tuple(preact.shape)}")
+            v, _, d.dy_pitch = _rows(dy, 0)
+            return d, C.byref(d), copy, wcopy, v is not dy, self._layer_ws(self.lib.ttc_linear_workspace, d, 1 if preact is None else 2)
+        pre_key = None if preact is None else (preact.shape, preact.dtype)
+        d, ref, copy, wcopy, dcopy, nb = self._layer_plan(
+            ("linear_bwd", x.shape, x.stride(), x.dtype, w.shape, w.stride(), w.dtype, dy.shape, dy.stride(), dy.dtype, activation, scale, pre_key), make)
+        bias = self._layer_vec(bias, d.cout, what + ": bias")
+        wshape = w.shape
+        if copy:
+            x = x.contiguous()
+        if wcopy:
+            w = w.contiguous()
+        if dcopy:
+            dy = dy.contiguous()
+        if preact is not None:
             preact = preact.contiguous()
-        dy, _, d.dy_pitch = _rows(dy, 0)
-        dx = t.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
-        dw = t.empty(wshape, dtype=x.dtype, device=x.device) if want_dw else None
-        db = t.empty(d.cout, dtype=t.float32, device=x.device) if want_dbias else None
-        ws, nb = self._layer_ws(self.lib.ttc_linear_workspace, d, 1 if preact is None else 2, what)
+        dx = x.new_empty(x.shape) if want_dx else None
+        dw = x.new_empty(wshape) if want_dw else None
+        db = x.new_empty(d.cout, dtype=t.float32) if want_dbias else None
+        ws = x.new_empty(nb, dtype=t.uint8) if nb else None
         ptr = lambda a: None if a is None else a.data_ptr()      # noqa: E731
-        self._check(self.lib.ttc_linear_backward(self._h, C.byref(d), ptr(dy), ptr(x), ptr(w), ptr(bias), ptr(preact), ptr(dx), ptr(dw), ptr(db), ptr(ws), nb,
-                                                 self._stream()), "ttc_linear_backward")
+        self._check(self.lib.ttc_linear_backward(self._h, ref, dy.data_ptr(), x.data_ptr(), w.data_ptr(), ptr(bias), ptr(preact), ptr(dx), ptr(dw), ptr(db),
+                                                 ptr(ws), nb, self._layer_stream()), "ttc_linear_backward")
         return dx, dw, db
 
     # -- debug ----------------------------------------------------------------------------

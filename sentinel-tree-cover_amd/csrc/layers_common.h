@@ -63,17 +63,17 @@ __device__ __forceinline__ float act_of(float z) {
     if constexpr (ACT == TTC_ACT_GELU) { float e; return z * normal_cdf(z, &e); }
     return z;
 }
-// The sigmoid family through e = exp(-|z|), r = 1 / (1 + e): sigmoid(|z|) = r, sigmoid(-|z|) = e r, sigmoid' = e r^2 -- one exponential, one
-// reciprocal, and no 1 - s that cancels for large |z|.
+// sigmoid' and tanh' go through e = exp(-|z|), r = 1 / (1 + e): sigmoid' = e r^2 has no 1 - s that cancels for large |z|.  swish' = s (1 + z (1 - s))
+// may cancel: it is 1 where that happens.  These slopes are what bounds the 16-bit norm's backward pass (64 lanes a CU and clock, a quarter of
+// that for exp and rcp), so every instruction counts.
 template <int ACT>
 __device__ __forceinline__ float slope_of(float z) {
     if constexpr (ACT == TTC_ACT_RELU) return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
     if constexpr (ACT == TTC_ACT_GELU) { float e; const float c = normal_cdf(z, &e); return c + z * 0.39894228f * e; }
-    if constexpr (ACT == TTC_ACT_SWISH || ACT == TTC_ACT_SIGMOID || ACT == TTC_ACT_TANH) {
+    if constexpr (ACT == TTC_ACT_SWISH) { const float s = sigmoidf(z); return s * (1.0f + z * (1.0f - s)); }
+    if constexpr (ACT == TTC_ACT_SIGMOID || ACT == TTC_ACT_TANH) {
         const float e = __expf((ACT == TTC_ACT_TANH ? -2.0f : -1.0f) * fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e), er2 = e * r * r;
-        if constexpr (ACT == TTC_ACT_SIGMOID) return er2;
-        if constexpr (ACT == TTC_ACT_TANH) return 4.0f * er2;
-        return (z < 0.0f ? e * r : r) + z * er2;
+        return ACT == TTC_ACT_TANH ? 4.0f * er2 : er2;
     }
     return 1.0f;
 }

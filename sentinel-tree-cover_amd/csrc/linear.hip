@@ -57,6 +57,25 @@ template <> struct Mma<float> {
     }
 };
 
+// acc[i][j] += b[i] a[j]: the instructions of one accumulator are as far apart as there are accumulators (fp32: four per pair; back to back each waited
+// for the one before, 57600 x 256 -> 128: GEMMBEFORE us)
+template <class T, int I, int J>
+__device__ __forceinline__ void mma_block(f32x4 (&acc)[I][J], const typename Mma<T>::Frag (&b)[I], const typename Mma<T>::Frag (&a)[J]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < I; ++i)
+#pragma unroll
+                for (int j = 0; j < J; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[i][c], a[j][c], acc[i][j], 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int j = 0; j < J; ++j) acc[i][j] = Mma<T>::run(b[i], a[j], acc[i][j]);
+    }
+}
+
 // free index (inside a wave's extent) of fragment f, instruction row r.  16-bit, B: fragment pairs interleave so that a lane's 2 x 4 results are 8
 // consecutive columns.
 template <class T, bool PAIR>
@@ -90,35 +109,60 @@ __device__ __forceinline__ uint4 load_piece(const T* p, long left) {
     return v;
 }
 
-// the 16-byte pieces of a BF x BKE tile a thread moves, global -> registers -> LDS
+// drop the first `n` elements of 16 bytes (all of them for n >= VE), zeros come in
+template <class T>
+__device__ __forceinline__ uint4 drop_front(uint4 v, int n) {
+    const int bits = min(n, VE<T>) * 8 * (int)sizeof(T);
+    unsigned long lo = v.x | (unsigned long)v.y << 32, hi = v.z | (unsigned long)v.w << 32;
+    if (bits >= 64) { lo = hi; hi = 0; }
+    const int b = bits & 63;
+    if (b) { lo = lo >> b | hi << (64 - b); hi >>= b; }
+    if (bits >= 128) lo = 0;
+    return make_uint4((unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32));
+}
+
+// the 16-byte pieces of a BF x BKE tile a thread moves, global -> registers -> LDS.  Inside the array the loads are plain.  In an edge tile a piece that
+// sticks out of its row is read so that it ENDS with the row and shifted down, one wholly outside reads something valid and becomes zero: no
+// element-by-element path (rows shorter than 16 bytes apart).  The shift happens on the way to LDS, so that the loads stay in flight.
 template <class T, bool KC, int BF>
 struct Stage {
-    static constexpr int CNT = BF * 8 / NT;
+    static constexpr int CNT = BF * 8 / NT, PR = BF / VE<T>;
     uint4 v[CNT];
-    __device__ __forceinline__ void load(const T* p, long ld, long f0, long F, long k0, long k1, int tid) {
+    static __device__ __forceinline__ int line(int id) { return KC ? id >> 3 : id / PR; }                      // row of the tile as stored
+    static __device__ __forceinline__ int along(int id) { return (KC ? id & 7 : id % PR) * VE<T>; }            // first element in it
+    // rows [r0, R), elements [e0, E) of the array remain
+    static __device__ __forceinline__ bool edge(long r0, long R, long e0, long E) { return r0 + (KC ? BF : BKE<T>) > R || e0 + (KC ? BKE<T> : BF) > E; }
+    __device__ __forceinline__ void load(const T* p, long ld, long f0, long F, long k0, long K, int tid) {
+        const long r0 = KC ? f0 : k0, R = KC ? F : K, e0 = KC ? k0 : f0, E = KC ? K : F;
+        if (!edge(r0, R, e0, E)) {
+            p += r0 * ld + e0;
 #pragma unroll
-        for (int i = 0; i < CNT; ++i) {
-            const int id = tid + i * NT;
-            if (KC) {
-                const long f = f0 + (id >> 3), k = k0 + (id & 7) * VE<T>;
-                v[i] = load_piece(p + f * ld + k, f < F ? k1 - k : 0);
-            } else {
-                constexpr int PR = BF / VE<T>;
-                const long k = k0 + id / PR, f = f0 + (id % PR) * VE<T>;
-                v[i] = load_piece(p + k * ld + f, k < k1 ? F - f : 0);
+            for (int i = 0; i < CNT; ++i) __builtin_memcpy(&v[i], p + line(tid + i * NT) * ld + along(tid + i * NT), 16);
+        } else if (E >= VE<T>) {
+#pragma unroll
+            for (int i = 0; i < CNT; ++i)
+                __builtin_memcpy(&v[i], p + min(r0 + line(tid + i * NT), R - 1) * ld + min(e0 + along(tid + i * NT), E - VE<T>), 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < CNT; ++i) {
+                const long r = r0 + line(tid + i * NT), e = e0 + along(tid + i * NT);
+                v[i] = load_piece(p + r * ld + e, r < R ? E - e : 0);
             }
         }
     }
-    __device__ __forceinline__ void store(char* lds, int tid) const {
+    __device__ __forceinline__ void store(char* lds, long f0, long F, long k0, long K, int tid) const {
+        const long r0 = KC ? f0 : k0, R = KC ? F : K, e0 = KC ? k0 : f0, E = KC ? K : F;
+        const bool fix = edge(r0, R, e0, E) && E >= VE<T>;
 #pragma unroll
         for (int i = 0; i < CNT; ++i) {
             const int id = tid + i * NT;
-            if (KC) {
-                reinterpret_cast<uint4*>(lds)[kc_slot(id >> 3, id & 7)] = v[i];
-            } else {
-                constexpr int PR = BF / VE<T>;
-                *reinterpret_cast<uint4*>(lds + fc_byte<T, BF>(id / PR, (id % PR) * VE<T>)) = v[i];
+            uint4 t = v[i];
+            if (fix) {
+                const long e = e0 + along(id);
+                t = drop_front<T>(t, r0 + line(id) < R ? (int)(e - min(e, E - VE<T>)) : VE<T>);
             }
+            if (KC) reinterpret_cast<uint4*>(lds)[kc_slot(id >> 3, id & 7)] = t;
+            else *reinterpret_cast<uint4*>(lds + fc_byte<T, BF>(line(id), along(id))) = t;
         }
     }
 };
@@ -232,8 +276,8 @@ __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
         for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     sa.load(A, a.lda, m0, a.M, k0, k1, tid);
     sb.load(B, a.ldb, n0, a.N, k0, k1, tid);
-    sa.store(lds, tid);
-    sb.store(lds + 2 * ABYTES, tid);
+    sa.store(lds, m0, a.M, k0, k1, tid);
+    sb.store(lds + 2 * ABYTES, n0, a.N, k0, k1, tid);
     __syncthreads();
     int cur = 0;
     for (long k = k0; k < k1; k += BKE<T>, cur ^= 1) {
@@ -251,14 +295,11 @@ __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
             for (int j = 0; j < FM; ++j) fa[j] = frag<T, AKC, BM, false>(la, wm * WM, j, ks, lane);
 #pragma unroll
             for (int i = 0; i < FN; ++i) fb[i] = frag<T, BKC, BN, true>(lb, wn * WN, i, ks, lane);
-#pragma unroll
-            for (int i = 0; i < FN; ++i)
-#pragma unroll
-                for (int j = 0; j < FM; ++j) acc[i][j] = Mma<T>::run(fb[i], fa[j], acc[i][j]);
+            mma_block<T>(acc, fb, fa);
         }
         if (more) {                                // the other half was last read before the previous barrier
-            sa.store(lds + (cur ^ 1) * ABYTES, tid);
-            sb.store(lds + 2 * ABYTES + (cur ^ 1) * BBYTES, tid);
+            sa.store(lds + (cur ^ 1) * ABYTES, m0, a.M, k + BKE<T>, k1, tid);
+            sb.store(lds + 2 * ABYTES + (cur ^ 1) * BBYTES, n0, a.N, k + BKE<T>, k1, tid);
         }
         __syncthreads();
     }
@@ -339,18 +380,6 @@ __global__ __launch_bounds__(NT) void k_join(GemmArgs a, const float* __restrict
 // other wave: x goes from memory straight into fragments (a lane's 16 bytes ARE the fragment), the next rows' while this row's products run, and
 // only the weights sit in LDS, loaded once per workgroup.  16-row steps read KS * FN KB of LDS per KS KB of x: 1/6 of the LDS rate at the memory's.
 template <class T> constexpr int KSTEP = 4 * VE<T>;           // contracted elements of one fragment step: 32 or 16
-
-// drop the first `n` elements of 16 bytes (all of them for n >= VE), zeros come in
-template <class T>
-__device__ __forceinline__ uint4 drop_front(uint4 v, int n) {
-    const int bits = n * 8 * (int)sizeof(T);
-    unsigned long lo = v.x | (unsigned long)v.y << 32, hi = v.z | (unsigned long)v.w << 32;
-    if (bits >= 64) { lo = hi; hi = 0; }
-    const int b = bits & 63;
-    if (b) { lo = lo >> b | hi << (64 - b); hi >>= b; }
-    if (bits >= 128) lo = 0;
-    return make_uint4((unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32));
-}
 
 // 16 rows of an array: the wave's row 0 is a scalar base, a lane's place in them a 32-bit byte offset that never changes (the narrow kernels take pitches
 // up to 2^24 elements).  Rows past the last read the last row: nothing of them is stored or summed.
@@ -455,14 +484,17 @@ __global__ __launch_bounds__(NT) void k_narrow(GemmArgs a) {
         x.trim(K, q);
         int here = 0;
         asm volatile("" : "+v"(here));        // the weights are read from LDS for every 16 rows: kept in registers they cost a wave per SIMD (fp32 64 -> 64: 144 -> 135 us)
-        f32x4 acc[FN];
+        f32x4 acc[FN][1];
 #pragma unroll
-        for (int f = 0; f < FN; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int f = 0; f < FN; ++f) acc[f][0] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+        for (int s = 0; s < KS; ++s) {
+            typename Mma<T>::Frag fw[FN];
+            const typename Mma<T>::Frag fx[1] = {__builtin_bit_cast(typename Mma<T>::Frag, x.v[s])};
 #pragma unroll
-            for (int f = 0; f < FN; ++f)
-                acc[f] = Mma<T>::run(frag<T, false, NP, PAIR>(lw + here, 0, f, s, lane), __builtin_bit_cast(typename Mma<T>::Frag, x.v[s]), acc[f]);
+            for (int f = 0; f < FN; ++f) fw[f] = frag<T, false, NP, PAIR>(lw + here, 0, f, s, lane);
+            mma_block<T>(acc, fw, fx);
+        }
         const int left = (int)min(a.M - base, 16L);
 #pragma unroll
         for (int p = 0; p < NG; ++p) {
@@ -470,7 +502,7 @@ __global__ __launch_bounds__(NT) void k_narrow(GemmArgs a) {
 #pragma unroll
             for (int u = 0; u < NR; ++u)
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[u][i] = acc[V == 8 ? 2 * (NR * p + u) + i / 4 : NR * p + u][i & 3];
+                for (int i = 0; i < V; ++i) v[u][i] = acc[V == 8 ? 2 * (NR * p + u) + i / 4 : NR * p + u][0][i & 3];
             if constexpr (NR == 2) trade(v[0], v[1], hi);
             const int col = NR * p * 4 * V + c0;
 #pragma unroll
@@ -588,7 +620,7 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
                     for (int i = 0; i < V; ++i) db[p][i] += (float)dz[p][i];
                 }
             } else {
-                f32x4 z[FN];
+                f32x4 z[FN][1];
                 if (!FULL && a.z) {
 #pragma unroll
                     for (int p = 0; p < NS; ++p) {
@@ -596,16 +628,21 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
 #pragma unroll
                         for (int u = 0; u < V / 4; ++u) {
                             const uint4 t = load_piece(a.z + row * a.N + col + 4 * u, (long)cols - 4 * u);
-                            z[p * (V / 4) + u] = __builtin_bit_cast(f32x4, t);
+                            z[p * (V / 4) + u][0] = __builtin_bit_cast(f32x4, t);
                         }
                     }
                 } else {
 #pragma unroll
-                    for (int f = 0; f < FN; ++f) {
+                    for (int f = 0; f < FN; ++f)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) z[f][i] = bias[H16 ? f >> 1 : f][H16 ? 4 * (f & 1) + i : i];
+                        for (int i = 0; i < 4; ++i) z[f][0][i] = bias[H16 ? f >> 1 : f][H16 ? 4 * (f & 1) + i : i];
 #pragma unroll
-                        for (int s = 0; s < KS; ++s) z[f] = Mma<T>::run(frag<T, false, NP, true>(lw, 0, f, s, lane), __builtin_bit_cast(Frag, x[h].v[s]), z[f]);
+                    for (int s = 0; s < KS; ++s) {
+                        Frag fw[FN];
+                        const Frag fr[1] = {__builtin_bit_cast(Frag, x[h].v[s])};
+#pragma unroll
+                        for (int f = 0; f < FN; ++f) fw[f] = frag<T, false, NP, true>(lw, 0, f, s, lane);
+                        mma_block<T>(z, fw, fr);
                     }
                 }
 #pragma unroll
@@ -613,7 +650,7 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
                     const Frag dv = __builtin_bit_cast(Frag, d[h].v[p]);
                     float t[V], zz[V];
 #pragma unroll
-                    for (int i = 0; i < V; ++i) { t[i] = (float)dv[i]; zz[i] = z[H16 ? 2 * p + i / 4 : p][i & 3]; }
+                    for (int i = 0; i < V; ++i) { t[i] = (float)dv[i]; zz[i] = z[H16 ? 2 * p + i / 4 : p][0][i & 3]; }
                     slope_vec<V>(t, zz, a.act);
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
@@ -623,15 +660,17 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
                 }
             }
             if (a.dx) {
-                f32x4 o[FK];
+                f32x4 o[FK][1];
 #pragma unroll
-                for (int f = 0; f < FK; ++f) {
-                    o[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int f = 0; f < FK; ++f) o[f][0] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int p = 0; p < NS; ++p) {
-                        const uint4 t = *reinterpret_cast<const uint4*>(lw + fc_byte<T, NP>(free_of<T, true>(f, r), p * KSTEP<T> + q * V));
-                        o[f] = Mma<T>::run(__builtin_bit_cast(Frag, t), dz[p], o[f]);
-                    }
+                for (int p = 0; p < NS; ++p) {
+                    Frag fw[FK];
+                    const Frag fr[1] = {dz[p]};
+#pragma unroll
+                    for (int f = 0; f < FK; ++f)
+                        fw[f] = __builtin_bit_cast(Frag, *reinterpret_cast<const uint4*>(lw + fc_byte<T, NP>(free_of<T, true>(f, r), p * KSTEP<T> + q * V)));
+                    mma_block<T>(o, fw, fr);
                 }
                 const int hi = KS == 1 ? 0 : r >> 3;
 #pragma unroll
@@ -641,7 +680,7 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
                     for (int u = 0; u < (KS == 1 ? 1 : 2); ++u) {
                         T t[V];
 #pragma unroll
-                        for (int i = 0; i < V; ++i) t[i] = (T)(o[H16 ? 2 * (p + u) + i / 4 : p + u][i & 3] * a.scale);
+                        for (int i = 0; i < V; ++i) t[i] = (T)(o[H16 ? 2 * (p + u) + i / 4 : p + u][0][i & 3] * a.scale);
                         __builtin_memcpy(v[u], t, 16);
                     }
                     if constexpr (KS > 1) trade(v[0], v[1], hi);
@@ -677,12 +716,10 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
             Frag fx[FK];
 #pragma unroll
             for (int j = 0; j < FK; ++j) fx[j] = frag<T, false, KP, false>(lx, 0, j, 0, lane);
+            Frag fz[FN];
 #pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                const Frag fz = frag<T, false, NP, false>(lz, 0, i, 0, lane);
-#pragma unroll
-                for (int j = 0; j < FK; ++j) dw[i][j] = Mma<T>::run(fz, fx[j], dw[i][j]);
-            }
+            for (int i = 0; i < FN; ++i) fz[i] = frag<T, false, NP, false>(lz, 0, i, 0, lane);
+            mma_block<T>(dw, fz, fx);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
@@ -783,19 +820,23 @@ __global__ void k_fill0(T* p, long n) {
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------------
 int bn_of(long N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }       // column tile: narrower only where the wide one would be mostly padding
-// how many ways the contracted index is split: one where the tiles fill the 256 CUs; else so that about two workgroups per CU run, each with at
-// least `least` of it, and the partials stay under 64 MB
+// row tile: 64 rows where 128 would leave CUs without a tile (5003 x 93 -> 177: 8.7 -> 6.2 us; but 8192 x 1024 -> 4096: 133 -> 159, twice the reads of w)
+int bm_of(long M, long N) { return bn_of(N) == 128 && ((M + 127) / 128) * ((N + 127) / 128) < 256 ? 64 : 128; }
+// how many ways the contracted index is split: one where the tiles fill the 256 CUs; else so that about that many workgroups run, each with at least
+// `least` of it, and the partials stay under 64 MB
 int gemm_splits(long M, long N, long K, long least) {
-    const long tiles = ((M + 127) / 128) * ((N + bn_of(N) - 1) / bn_of(N));
+    const long bm = bm_of(M, N), tiles = ((M + bm - 1) / bm) * ((N + bn_of(N) - 1) / bn_of(N));
     const long fit = std::max<long>(1, (64L << 20) / (M * N * 4));
-    return (int)std::max<long>(1, std::min<long>({512 / tiles, K / least, fit}));
+    return (int)std::max<long>(1, std::min<long>({256 / tiles, K / least, fit}));
 }
-constexpr long LEAST_K = 128, LEAST_ROWS = 512;
+constexpr long LEAST_K = 128, LEAST_ROWS = 128;
 
 template <class T>
 void join_launch(const GemmArgs& a, const float* part, long rec, int splits, int tail, float* tail_out, hipStream_t s) {
     const long vecs = a.M * ((a.N + 3) / 4) + (tail + 3) / 4;
-    if (splits > 16) hipLaunchKernelGGL((k_join<T, 16>), dim3((unsigned)((vecs + 15) / 16)), dim3(NT), 0, s, a, part, rec, splits, tail, tail_out);
+    // more lanes on the splits where there are few outputs to spread over the chip
+    if (splits > 128 && vecs < 2048) hipLaunchKernelGGL((k_join<T, 64>), dim3((unsigned)((vecs + 3) / 4)), dim3(NT), 0, s, a, part, rec, splits, tail, tail_out);
+    else if (splits > 16) hipLaunchKernelGGL((k_join<T, 16>), dim3((unsigned)((vecs + 15) / 16)), dim3(NT), 0, s, a, part, rec, splits, tail, tail_out);
     else hipLaunchKernelGGL((k_join<T, 1>), dim3((unsigned)((vecs + NT - 1) / NT)), dim3(NT), 0, s, a, part, rec, splits, tail, tail_out);
 }
 
@@ -809,12 +850,13 @@ void gemm_launch(GemmArgs a, int splits, float* ws, hipStream_t s) {
         splits = (int)((a.K + a.k_per - 1) / a.k_per);
     }
     if (splits > 1) { a.C = ws; a.partial = 1; }
-    a.mt = (int)((a.M + 127) / 128);
-    const int bn = bn_of(a.N);
+    const int bn = bn_of(a.N), bm = bm_of(a.M, a.N);
+    a.mt = (int)((a.M + bm - 1) / bm);
     a.nt = (a.N + bn - 1) / bn;
     auto go = [&](auto fn) { hipLaunchKernelGGL(fn, dim3((unsigned)(a.mt * a.nt), splits), dim3(NT), 0, s, a); };
     if (bn == 32) go(k_gemm<T, AKC, BKC, 128, 32, 4>);
     else if (bn == 64) go(k_gemm<T, AKC, BKC, 128, 64, 2>);
+    else if (bm == 64) go(k_gemm<T, AKC, BKC, 64, 128, 1>);
     else go(k_gemm<T, AKC, BKC, 128, 128, 2>);
     if (splits > 1) join_launch<T>(j, ws, a.M * a.N, splits, 0, nullptr, s);
 }

@@ -357,8 +357,11 @@ def test_refusals_on_the_device(ctx):
     import ctypes as C
     from ttc import _lib
     lib, p = ctx.lib, x.data_ptr()
-    d = _lib.TTCGroupNormDesc(0, 0, 1, 6, 16, 4, 96, 16, 1e-5)
+    d = _lib.TTCGroupNormDesc(0, 0, 1, 1 << 20, 16, 4, 96, 16, 1e-5)         # long enough to need scratch memory
     assert lib.ttc_group_norm(ctx._h, C.byref(d), p, None, None, p, None, p, 8, None) == 1 and b"workspace" in lib.ttc_last_error(ctx._h)
+    assert lib.ttc_group_norm(ctx._h, C.byref(d), None, None, None, p, None, p, 1 << 20, None) == 1
+    assert lib.ttc_group_norm_backward(ctx._h, C.byref(d), p, 96, 16, p, None, None, p, p, None, None, p, 8, None) == 1 and b"workspace" in lib.ttc_last_error(ctx._h)
+    d = _lib.TTCGroupNormDesc(0, 0, 1, 6, 16, 4, 96, 16, 1e-5)
     assert lib.ttc_group_norm(ctx._h, C.byref(d), None, None, None, p, None, p, 1 << 20, None) == 1
     assert lib.ttc_group_norm_backward(ctx._h, C.byref(d), p, 96, 16, p, None, None, None, p, None, None, p, 1 << 20, None) == 1
     l = _lib.TTCLinearDesc(0, 2, 6, 16, 8, 16, 8, 8, 8, 1.0)

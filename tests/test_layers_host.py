@@ -52,8 +52,10 @@ def test_group_norm_descriptor_refusals(lib, bad):
 
 def test_group_norm_descriptor_accepts(lib):
     for kw in (dict(), dict(rows=1, x_pitch=0), dict(n=1, x_stride=0), dict(channels=4096, groups=4096, x_pitch=4096), dict(eps=0.0), dict(dtype=2), dict(dtype=3)):
-        st, nb = _norm(lib, **kw)
-        assert st == 0 and nb > 0, kw
+        assert _norm(lib, **kw)[0] == 0 and _norm(lib, 1, **kw)[0] == 0, kw
+    for backward in (0, 1):
+        st, nb = _norm(lib, backward, rows=1 << 20)                       # long samples need scratch memory
+        assert st == 0 and nb > 0
     assert _norm(lib, n=0) == (0, 0) and _norm(lib, rows=0) == (0, 0)
     assert lib.ttc_group_norm_workspace(None, 0, C.byref(C.c_size_t())) == 1
     assert lib.ttc_group_norm_workspace(C.byref(_lib.TTCGroupNormDesc(**NORM)), 0, None) == 1
@@ -101,13 +103,24 @@ def test_binding_refusals(host):
         with pytest.raises(ValueError, match="linear"):
             host._linear_desc(bx, bw, None, 1.0, "linear")
     with pytest.raises(ValueError, match=r"gamma must be \[16\]"):
-        host._norm_desc(x, torch.ones(8), None, 4, 1e-5, None, "group_norm")
+        host._layer_vec(torch.ones(8), 16, "group_norm: gamma")
     with pytest.raises(ValueError, match=r"\[n, ..., channels\]"):
-        host._norm_desc(x[0, 0], None, None, 4, 1e-5, None, "group_norm")
+        host._norm_plan(x[0, 0], 4, 1e-5, None, "group_norm", 0)
     # TF kernel shape, transposed weight copied, strided weight read in place
-    _, w2, d = host._linear_desc(x, torch.zeros(1, 1, 16, 8), "relu", 0.1, "linear")
-    assert (d.rows, d.cin, d.cout, d.x_pitch, d.w_pitch, d.activation) == (24, 16, 8, 16, 8, 1) and tuple(w2.shape) == (16, 8)
-    _, w2, d = host._linear_desc(x, torch.zeros(16, 20)[:, 3:11], None, 1.0, "linear")
-    assert d.w_pitch == 20
-    _, w2, d = host._linear_desc(x, torch.zeros(8, 16).t(), None, 1.0, "linear")
-    assert d.w_pitch == 8 and w2.is_contiguous()
+    d, copy, wcopy, shape = host._linear_desc(x, torch.zeros(1, 1, 16, 8), "relu", 0.1, "linear")
+    assert (d.rows, d.cin, d.cout, d.x_pitch, d.w_pitch, d.activation) == (24, 16, 8, 16, 8, 1) and not copy and not wcopy and shape == (4, 6, 8)
+    d, copy, wcopy, _ = host._linear_desc(x, torch.zeros(16, 20)[:, 3:11], None, 1.0, "linear")
+    assert d.w_pitch == 20 and not wcopy
+    d, copy, wcopy, _ = host._linear_desc(x, torch.zeros(8, 16).t(), None, 1.0, "linear")
+    assert d.w_pitch == 8 and wcopy
+    assert host._layer_vec(torch.ones(16, dtype=torch.float64)[::2], 8, "p").dtype == torch.float32
+
+
+def test_plans_are_kept_by_shape_alone_and_bounded(host):
+    made = []
+    for i in range(10000):
+        host._layer_plan(("k", i % 5000), lambda: made.append(i) or i)
+    assert len(host._plans) <= 4096
+    n = len(made)
+    host._layer_plan(("k", 4999), lambda: made.append(0))
+    assert len(made) == n
