@@ -252,6 +252,37 @@ __device__ __forceinline__ void emit(const GemmArgs& a, long row, int col, int l
     }
 }
 
+// a wave's accumulators (FN fragments of columns, FM of rows) from row m0, column n0
+template <class T, int FN, int FM>
+__device__ __forceinline__ void store_tile(const GemmArgs& a, f32x4 (&acc)[FN][FM], long m0, int n0, int lane) {
+    constexpr int WN = FN * 16;
+    const int r = lane & 15, q = lane >> 4, hi = r >> 3;
+    constexpr int V = VE<T>, NV = WN / (4 * V);               // columns a lane stores at once, such runs of a wave
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const long base = m0 + j * 16;
+#pragma unroll
+        for (int p = 0; p < NV; p += 2) {
+            float v[2][V];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                if (p + u < NV)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[u][i] = acc[V == 8 ? 2 * (p + u) + i / 4 : p + u][j][i & 3];
+            if (p + 1 < NV) trade(v[0], v[1], hi);
+            const int col = n0 + (p + (p + 1 < NV ? hi : 0)) * 4 * V + q * V;
+            if (col >= a.N) continue;
+            if (p + 1 < NV) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if (base + (r & 7) + 8 * u < a.M) emit<T, V>(a, base + (r & 7) + 8 * u, col, a.N - col, v[u]);
+            } else if (base + r < a.M) {
+                emit<T, V>(a, base + r, col, a.N - col, v[0]);
+            }
+        }
+    }
+}
+
 // ---- the tile kernel --------------------------------------------------------------------------------------------------------------------
 template <class T, bool AKC, bool BKC, int BM, int BN, int WGM>
 __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
@@ -303,31 +334,86 @@ __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
         }
         __syncthreads();
     }
-    const int r = lane & 15, q = lane >> 4, hi = r >> 3;
-    constexpr int V = VE<T>, NV = WN / (4 * V);               // columns a lane stores at once, such runs of a wave
+    store_tile<T>(a, acc, m0 + wm * WM, n0 + wn * WN, lane);
+}
+
+// ---- the wide tile kernel: 16-bit operands, 256 x 256 -------------------------------------------------------------------------------------
+// One workgroup of 8 waves per CU (2 x 4, 128 x 64 outputs each: 24 KB of LDS fragments per wave and step against 64 matrix instructions, 3/4 of the
+// LDS rate), two 64 KB stages.  Tiles go from memory to LDS without passing registers, 16 bytes a lane; the swizzle is in which piece of its row a
+// lane fetches.  A stage is fetched while the other is multiplied; one barrier a step.  Rows and columns past the array fetch the last ones (not stored);
+// the contracted range is a multiple of 64 and every row 16-byte aligned: other calls take k_gemm.
+// The copy is written out because the compiler, which cannot tell the stages apart, waits for every copy in flight before each LDS read.  It has no
+// register result; the wait for it is the explicit one in front of the barrier.
+template <class T, bool KC>
+struct WideTile {
+    unsigned off[4];                               // a lane's pieces, bytes from the step's base
+    __device__ __forceinline__ void init(long ld, long f0, long F, int wave, int lane) {
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-        const long base = m0 + wm * WM + j * 16;
-#pragma unroll
-        for (int p = 0; p < NV; p += 2) {
-            float v[2][V];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-                if (p + u < NV)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) v[u][i] = acc[V == 8 ? 2 * (p + u) + i / 4 : p + u][j][i & 3];
-            if (p + 1 < NV) trade(v[0], v[1], hi);
-            const int col = n0 + wn * WN + (p + (p + 1 < NV ? hi : 0)) * 4 * V + q * V;
-            if (col >= a.N) continue;
-            if (p + 1 < NV) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    if (base + (r & 7) + 8 * u < a.M) emit<T, V>(a, base + (r & 7) + 8 * u, col, a.N - col, v[u]);
-            } else if (base + r < a.M) {
-                emit<T, V>(a, base + r, col, a.N - col, v[0]);
+        for (int i = 0; i < 4; ++i) {
+            const int id = (i * 8 + wave) * 64 + lane;
+            if (KC) {
+                const int row = id >> 3, ch = (id & 7) ^ ((row ^ (row >> 3)) & 7);
+                off[i] = (unsigned)min((long)row, F - 1 - f0) * (unsigned)(ld * 2) + ch * 16;
+            } else {
+                const int k = id >> 5, c = id & 31, sw = (k & 3) | ((k >> 1) & 4);
+                off[i] = (unsigned)k * (unsigned)(ld * 2) + (unsigned)min((long)(((c >> 1) ^ sw) * 16 + (c & 1) * 8), F - 8 - f0) * 2;
             }
         }
     }
+    __device__ __forceinline__ void fetch(const T* p, long ld, long f0, long k, unsigned lds, int wave) const {
+        const T* base = KC ? p + f0 * ld + k : p + k * ld + f0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds + (i * 8 + wave) * 1024u), "v"(off[i]), "s"(base) : "memory", "m0");
+    }
+};
+template <class T, bool AKC, bool BKC>
+__global__ __launch_bounds__(512) void k_gemm_wide(GemmArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char wide_lds[];      // A0 A1 B0 B1, 32 KB each
+    constexpr int TB = 256 * 128;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
+    const int total = a.mt * a.nt, bid = blockIdx.x, xcd = bid & 7, per = total >> 3, rem = total & 7;
+    const int tile = xcd * per + min(xcd, rem) + (bid >> 3);
+    const long m0 = (long)(tile / a.nt) * 256;
+    const int n0 = (tile % a.nt) * 256;
+    const long k0 = blockIdx.y * a.k_per, k1 = min(k0 + a.k_per, a.K);
+    const T* A = (const T*)a.A;
+    const T* B = (const T*)a.B;
+    f32x4 acc[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)wide_lds;
+    WideTile<T, AKC> ta;
+    WideTile<T, BKC> tb;
+    ta.init(a.lda, m0, a.M, wave, lane);
+    tb.init(a.ldb, n0, a.N, wave, lane);
+    ta.fetch(A, a.lda, m0, k0, lds0, wave);
+    tb.fetch(B, a.ldb, n0, k0, lds0 + 2 * TB, wave);
+    __builtin_amdgcn_s_waitcnt(0x0f70);            // vmcnt(0): this wave's pieces have landed; the barrier makes that everyone's
+    __syncthreads();
+    int cur = 0;
+    for (long k = k0; k < k1; k += 64, cur ^= 1) {
+        if (k + 64 < k1) {                         // the other stage was last read before the barrier
+            ta.fetch(A, a.lda, m0, k + 64, lds0 + (cur ^ 1) * TB, wave);
+            tb.fetch(B, a.ldb, n0, k + 64, lds0 + (2 + (cur ^ 1)) * TB, wave);
+        }
+        const char* la = wide_lds + cur * TB;
+        const char* lb = wide_lds + (2 + cur) * TB;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            typename Mma<T>::Frag fa[8], fb[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fb[i] = frag<T, BKC, 256, true>(lb, wn * 64, i, ks, lane);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) fa[j] = frag<T, AKC, 256, false>(la, wm * 128, j, ks, lane);
+            mma_block<T>(acc, fb, fa);
+        }
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+        __syncthreads();
+    }
+    store_tile<T>(a, acc, m0 + wm * 128, n0 + wn * 64, lane);
 }
 
 // ---- joining the splits of the contracted index: C = epilogue(sum of the partials), 4 columns a thread, L lanes over the splits -------------------
@@ -822,6 +908,9 @@ __global__ void k_fill0(T* p, long n) {
 int bn_of(long N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }       // column tile: narrower only where the wide one would be mostly padding
 // row tile: 64 rows where 128 would leave CUs without a tile (5003 x 93 -> 177: 8.7 -> 6.2 us; but 8192 x 1024 -> 4096: 133 -> 159, twice the reads of w)
 int bm_of(long M, long N) { return bn_of(N) == 128 && ((M + 127) / 128) * ((N + 127) / 128) < 256 ? 64 : 128; }
+// the 256 x 256 kernel: where its tiles fill the CUs, or would with the contracted index split
+constexpr long WIDE_PITCH = 1L << 22;                         // 256 rows of them fit a 32-bit byte offset
+bool wide_ok(long M, long N, long K) { return K % 64 == 0 && M >= 256 && N >= 256 && ((M + 255) / 256) * ((N + 255) / 256) * std::max<long>(1, K / 1024) >= 192; }
 // how many ways the contracted index is split: one where the tiles fill the 256 CUs; else so that about that many workgroups run, each with at least
 // `least` of it, and the partials stay under 64 MB
 int gemm_splits(long M, long N, long K, long least) {
@@ -850,6 +939,19 @@ void gemm_launch(GemmArgs a, int splits, float* ws, hipStream_t s) {
         splits = (int)((a.K + a.k_per - 1) / a.k_per);
     }
     if (splits > 1) { a.C = ws; a.partial = 1; }
+    if constexpr (sizeof(T) == 2) {
+        if (wide_ok(a.M, a.N, a.K) && a.lda % 8 == 0 && a.ldb % 8 == 0 && a.lda <= WIDE_PITCH && a.ldb <= WIDE_PITCH && (uintptr_t)a.A % 16 == 0 && (uintptr_t)a.B % 16 == 0 && (AKC || a.M % 8 == 0)
+            && (BKC || a.N % 8 == 0)) {
+            static LdsConfig cfg;
+            if (cfg.ensure(k_gemm_wide<T, AKC, BKC>, 4 * 256 * 128) == hipSuccess) {
+                a.mt = (int)((a.M + 255) / 256);
+                a.nt = (a.N + 255) / 256;
+                hipLaunchKernelGGL((k_gemm_wide<T, AKC, BKC>), dim3((unsigned)(a.mt * a.nt), splits), dim3(512), 4 * 256 * 128, s, a);
+                if (splits > 1) join_launch<T>(j, ws, a.M * a.N, splits, 0, nullptr, s);
+                return;
+            }
+        }
+    }
     const int bn = bn_of(a.N), bm = bm_of(a.M, a.N);
     a.mt = (int)((a.M + bm - 1) / bm);
     a.nt = (a.N + bn - 1) / bn;

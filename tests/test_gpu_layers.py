@@ -260,6 +260,24 @@ def test_linear(ctx, dtype, shape):
                  randn((m, n), dt, 150 + i) if i % 2 else None, act, scale=(1.0, 0.1)[i // 2 % 2], dy=randn((m, n), dt, 200 + i))
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("shape", [(3333, 128, 3848), (3333, 3848, 128), (192, 3336, 3848), (1000, 12352, 1000), (3584, 64, 4096)], ids=str)
+def test_linear_wide(ctx, dtype, shape):
+    """16-bit products of many 256 x 256 tiles, ragged at the far edges: in y, in dx, in dw, with the contracted index split; the strided and the
+    misaligned call give the aligned call's bits or stay within the bounds"""
+    m, k, n = shape
+    dt = DT[dtype]
+    x, w, dy = randn((m, k), dt, 1), randn((k, n), dt, 2, k ** -0.5), randn((m, n), dt, 3)
+    bias, res = randn((n,), torch.float32, 4, 0.3), randn((m, n), dt, 5)
+    y = check_linear(ctx, x, w, bias, res, "swish", scale=0.5, dy=dy)
+    ws, xs = randn((k, n + 24), dt, 6)[:, 8:n + 8], randn((m, k + 16), dt, 7)[:, 16:]
+    ws.copy_(w), xs.copy_(x)
+    assert torch.equal(y, ctx.linear(xs, ws, bias, res, activation="swish", scale=0.5))
+    off = randn((m, k + 3), dt, 8)[:, 3:]
+    off.copy_(x)
+    check_linear(ctx, off, w, bias, res, "swish", scale=0.5)
+
+
 @pytest.mark.parametrize("rows", list(range(1, 19)) + [31, 33, 63, 65])
 def test_linear_row_counts(ctx, rows):
     """every count of a few rows, which take paths of their own, at sizes with and without whole vectors"""
