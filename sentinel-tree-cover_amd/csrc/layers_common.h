@@ -41,16 +41,16 @@ __device__ __forceinline__ float tanh_rel(float v) {
     return fabsf(v) < 0.5f ? p : e;
 }
 
-// Normal distribution function of z and e = exp(-z^2 / 2).  cdf(-|z|) = erfc(x) / 2 with x = |z| / sqrt 2, and erfc(x) = exp(-x^2) t P(t),
+// h = normal distribution function of -|z|, and e = exp(-z^2 / 2).  h = erfc(x) / 2 with x = |z| / sqrt 2, and erfc(x) = exp(-x^2) t P(t),
 // t = 1 / (1 + 0.356 x): P is the degree-9 Chebyshev fit of exp(x^2) erfc(x) / t over t in (0, 1], 2.7e-8 of its value everywhere (0.356 minimises
-// that).  No 1 + erf: the negative tail keeps its relative accuracy.  A quarter of the registers of the library's erfc, which set the kernels' occupancy.
-__device__ __forceinline__ float normal_cdf(float z, float* e) {
+// that; P is halved below).  No 1 + erf: the negative tail keeps its relative accuracy.  A quarter of the registers of the library's erfc, which set
+// the kernels' occupancy.
+__device__ __forceinline__ float normal_tail(float z, float* e) {
     const float az = fabsf(z), t = __builtin_amdgcn_rcpf(1.0f + (0.356f * 0.70710678f) * az);
-    const float p = 0.20085149f + t * (0.20085289f + t * (0.18806472f + t * (0.16363163f + t * (0.11904900f + t * (0.12201817f
-                    + t * (-0.05494823f + t * (0.17837204f + t * (-0.15755503f + t * 0.03966334f))))))));
+    const float p = 0.100425743f + t * (0.100426443f + t * (0.094032362f + t * (0.081815816f + t * (0.0595245f + t * (0.061009083f
+                    + t * (-0.027474117f + t * (0.08918602f + t * (-0.078777514f + t * 0.01983167f))))))));
     *e = __expf(-0.5f * z * z);
-    const float h = 0.5f * t * p * *e;
-    return z < 0.0f ? h : 1.0f - h;
+    return t * p * *e;
 }
 
 // act(z) / act'(z) of one element for a fixed activation
@@ -60,7 +60,7 @@ __device__ __forceinline__ float act_of(float z) {
     if constexpr (ACT == TTC_ACT_SWISH) return z * sigmoidf(z);
     if constexpr (ACT == TTC_ACT_SIGMOID) return sigmoidf(z);
     if constexpr (ACT == TTC_ACT_TANH) return tanh_rel(z);
-    if constexpr (ACT == TTC_ACT_GELU) { float e; return z * normal_cdf(z, &e); }
+    if constexpr (ACT == TTC_ACT_GELU) { float e; const float h = normal_tail(z, &e); return z * (z < 0.0f ? h : 1.0f - h); }
     return z;
 }
 // sigmoid' and tanh' go through e = exp(-|z|), r = 1 / (1 + e): sigmoid' = e r^2 has no 1 - s that cancels for large |z|.  swish' = s (1 + z (1 - s))
@@ -69,7 +69,7 @@ __device__ __forceinline__ float act_of(float z) {
 template <int ACT>
 __device__ __forceinline__ float slope_of(float z) {
     if constexpr (ACT == TTC_ACT_RELU) return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
-    if constexpr (ACT == TTC_ACT_GELU) { float e; const float c = normal_cdf(z, &e); return c + z * 0.39894228f * e; }
+    if constexpr (ACT == TTC_ACT_GELU) { float e; const float h = normal_tail(z, &e); return (z < 0.0f ? h : 1.0f - h) + z * 0.39894228f * e; }
     if constexpr (ACT == TTC_ACT_SWISH) { const float s = sigmoidf(z); return s * (1.0f + z * (1.0f - s)); }
     if constexpr (ACT == TTC_ACT_SIGMOID || ACT == TTC_ACT_TANH) {
         const float e = __expf((ACT == TTC_ACT_TANH ? -2.0f : -1.0f) * fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e), er2 = e * r * r;

@@ -58,7 +58,7 @@ template <> struct Mma<float> {
 };
 
 // acc[i][j] += b[i] a[j]: the instructions of one accumulator are as far apart as there are accumulators (fp32: four per pair; back to back each waited
-// for the one before, 57600 x 256 -> 128: GEMMBEFORE us)
+// for the one before)
 template <class T, int I, int J>
 __device__ __forceinline__ void mma_block(f32x4 (&acc)[I][J], const typename Mma<T>::Frag (&b)[I], const typename Mma<T>::Frag (&a)[J]) {
     if constexpr (sizeof(T) == 4) {
@@ -252,32 +252,45 @@ __device__ __forceinline__ void emit(const GemmArgs& a, long row, int col, int l
     }
 }
 
-// a wave's accumulators (FN fragments of columns, FM of rows) from row m0, column n0
+// a wave's accumulators (FN fragments of columns, FM of rows) from row m0, column n0.  Columns outermost: a lane's bias is loaded once for all its rows.
 template <class T, int FN, int FM>
 __device__ __forceinline__ void store_tile(const GemmArgs& a, f32x4 (&acc)[FN][FM], long m0, int n0, int lane) {
-    constexpr int WN = FN * 16;
-    const int r = lane & 15, q = lane >> 4, hi = r >> 3;
-    constexpr int V = VE<T>, NV = WN / (4 * V);               // columns a lane stores at once, such runs of a wave
+    const int r = lane & 15, q = lane >> 4;
+    constexpr int V = VE<T>, NV = FN * 16 / (4 * V), NR = NV == 1 ? 1 : 2;      // columns a lane stores at once, such runs of a wave, rows of each
+    const int hi = NR == 1 ? 0 : r >> 3, r0 = NR == 1 ? r : r & 7;
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-        const long base = m0 + j * 16;
+    for (int p = 0; p < NV; p += NR) {
+        const int col = n0 + (p + hi) * 4 * V + q * V, left = a.N - col;
+        float bias[V];
 #pragma unroll
-        for (int p = 0; p < NV; p += 2) {
-            float v[2][V];
+        for (int i = 0; i < V; ++i) bias[i] = 0.0f;
+        if (a.fwd && a.bias && left > 0) load_part<float, V>(a.bias + col, left, bias);
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-                if (p + u < NV)
+        for (int j = 0; j < FM; ++j) {
+            float v[NR][V];
 #pragma unroll
-                    for (int i = 0; i < V; ++i) v[u][i] = acc[V == 8 ? 2 * (p + u) + i / 4 : p + u][j][i & 3];
-            if (p + 1 < NV) trade(v[0], v[1], hi);
-            const int col = n0 + (p + (p + 1 < NV ? hi : 0)) * 4 * V + q * V;
-            if (col >= a.N) continue;
-            if (p + 1 < NV) {
+            for (int u = 0; u < NR; ++u)
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    if (base + (r & 7) + 8 * u < a.M) emit<T, V>(a, base + (r & 7) + 8 * u, col, a.N - col, v[u]);
-            } else if (base + r < a.M) {
-                emit<T, V>(a, base + r, col, a.N - col, v[0]);
+                for (int i = 0; i < V; ++i) v[u][i] = acc[V == 8 ? 2 * (p + u) + i / 4 : p + u][j][i & 3];
+            if constexpr (NR == 2) trade(v[0], v[1], hi);
+            if (left <= 0) continue;
+#pragma unroll
+            for (int u = 0; u < NR; ++u) {
+                const long row = m0 + j * 16 + r0 + 8 * u;
+                if (row >= a.M) continue;
+                if (a.partial) {
+                    store_part<float, V>((float*)a.C + ((long)blockIdx.y * a.M + row) * a.N + col, left, v[u]);
+                } else if (!a.fwd) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[u][i] *= a.alpha;
+                    store_part<T, V>((T*)a.C + row * a.ldc + col, left, v[u]);
+                } else {
+                    float res[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) res[i] = 0.0f;
+                    if (a.res) load_part<T, V>((const T*)a.res + row * a.ldr + col, left, res);
+                    finish<T, V>(a, row, col, left, v[u], bias, res);
+                }
             }
         }
     }
@@ -908,15 +921,18 @@ __global__ void k_fill0(T* p, long n) {
 int bn_of(long N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }       // column tile: narrower only where the wide one would be mostly padding
 // row tile: 64 rows where 128 would leave CUs without a tile (5003 x 93 -> 177: 8.7 -> 6.2 us; but 8192 x 1024 -> 4096: 133 -> 159, twice the reads of w)
 int bm_of(long M, long N) { return bn_of(N) == 128 && ((M + 127) / 128) * ((N + 127) / 128) < 256 ? 64 : 128; }
-// the 256 x 256 kernel: where its tiles fill the CUs, or would with the contracted index split
+// the 256 x 256 kernel: where its tiles fill the CUs, or do with the contracted index split into runs of at least 1024
 constexpr long WIDE_PITCH = 1L << 22;                         // 256 rows of them fit a 32-bit byte offset
-bool wide_ok(long M, long N, long K) { return K % 64 == 0 && M >= 256 && N >= 256 && ((M + 255) / 256) * ((N + 255) / 256) * std::max<long>(1, K / 1024) >= 192; }
-// how many ways the contracted index is split: one where the tiles fill the 256 CUs; else so that about that many workgroups run, each with at least
-// `least` of it, and the partials stay under 64 MB
-int gemm_splits(long M, long N, long K, long least) {
-    const long bm = bm_of(M, N), tiles = ((M + bm - 1) / bm) * ((N + bn_of(N) - 1) / bn_of(N));
+long wide_tiles(long M, long N) { return ((M + 255) / 256) * ((N + 255) / 256); }
+bool wide_ok(long M, long N, long K) { return K % 64 == 0 && M >= 256 && N >= 256 && wide_tiles(M, N) * std::max<long>(1, K / 1024) >= 192; }
+// how many ways the contracted index is split: one where the tiles fill the CUs; else so that one workgroup per CU runs, two where the index is long
+// (4096 x 1024 -> 1024 bf16: y 23 us with one, 34 with two; dw of 65536 x 512 -> 256: 76 us with one, 56 with two), each with at least `least` of it,
+// and the partials stay under 64 MB
+int gemm_splits(long M, long N, long K, long least, int bytes) {
     const long fit = std::max<long>(1, (64L << 20) / (M * N * 4));
-    return (int)std::max<long>(1, std::min<long>({256 / tiles, K / least, fit}));
+    if (bytes == 2 && wide_ok(M, N, K)) return (int)std::max<long>(1, std::min<long>({256 / wide_tiles(M, N), K / 1024, fit}));
+    const long bm = bm_of(M, N), tiles = ((M + bm - 1) / bm) * ((N + bn_of(N) - 1) / bn_of(N));
+    return (int)std::max<long>(1, std::min<long>({(K > 4096 ? 512 : 256) / tiles, K / least, fit}));
 }
 constexpr long LEAST_K = 128, LEAST_ROWS = 128;
 
@@ -963,13 +979,14 @@ void gemm_launch(GemmArgs a, int splits, float* ws, hipStream_t s) {
     if (splits > 1) join_launch<T>(j, ws, a.M * a.N, splits, 0, nullptr, s);
 }
 
-// the narrow kernels: weights of at most 64 KB as an LDS image whose padded sides are powers of two of 16-byte steps
+// the narrow kernels: weights of at most 32 KB as an LDS image whose padded sides are powers of two of 16-byte steps (57600 x 256 -> 128 bf16, 64 KB:
+// 32 us against 15 by tiles)
 int pow2_at_least(int v) { int p = 1; while (p < v) p *= 2; return p; }
 constexpr long NARROW_PITCH = 1L << 24;                       // 15 rows of them fit a 32-bit byte offset
 bool narrow_fwd(const ttc_linear_desc* d) {
     if (d->x_pitch > NARROW_PITCH || d->res_pitch > NARROW_PITCH) return false;
     const int step = d->dtype == TTC_DT_F32 ? 16 : 32;
-    return d->cin <= 8 * step && d->cout <= 128;
+    return d->cin <= 8 * step && d->cout <= 128 && pow2_at_least((d->cin + step - 1) / step) * pow2_at_least((d->cout + 15) / 16) <= 32;
 }
 bool narrow_bwd(const ttc_linear_desc* d) {
     if (d->x_pitch > NARROW_PITCH || d->dy_pitch > NARROW_PITCH) return false;
@@ -1038,9 +1055,9 @@ BwdWs linear_ws(const ttc_linear_desc* d, bool have_z) {
     w.dz = act && !have_z ? up(cells * sizeof(float)) : 0;
     w.sums = w.dz + (act ? up(cells * dtype_bytes(d->dtype)) : 0);
     w.part = w.sums + up((size_t)w.blocks * d->cout * sizeof(float));
-    const size_t zs = act && !have_z ? (size_t)gemm_splits(d->rows, d->cout, d->cin, LEAST_K) : 1;
-    w.dx_splits = gemm_splits(d->rows, d->cin, d->cout, LEAST_K);
-    w.dw_splits = gemm_splits(d->cin, d->cout, d->rows, LEAST_ROWS);
+    const size_t zs = act && !have_z ? (size_t)gemm_splits(d->rows, d->cout, d->cin, LEAST_K, dtype_bytes(d->dtype)) : 1;
+    w.dx_splits = gemm_splits(d->rows, d->cin, d->cout, LEAST_K, dtype_bytes(d->dtype));
+    w.dw_splits = gemm_splits(d->cin, d->cout, d->rows, LEAST_ROWS, dtype_bytes(d->dtype));
     size_t part = 0;
     if (zs > 1) part = zs * cells;
     if (w.dx_splits > 1) part = std::max(part, (size_t)w.dx_splits * d->rows * d->cin);
@@ -1105,7 +1122,7 @@ ttc_status ttc_linear_workspace(const ttc_linear_desc* d, int32_t backward, size
     if (linear_check(d)) return TTC_ERR_ARG;
     if (d->rows == 0) return TTC_OK;
     if (backward) { *bytes = linear_ws(d, backward == TTC_LINEAR_HAVE_PREACT).total; return TTC_OK; }
-    const int sp = narrow_fwd(d) ? 1 : gemm_splits(d->rows, d->cout, d->cin, LEAST_K);
+    const int sp = narrow_fwd(d) ? 1 : gemm_splits(d->rows, d->cout, d->cin, LEAST_K, dtype_bytes(d->dtype));
     if (sp > 1) *bytes = (size_t)sp * d->rows * d->cout * sizeof(float);
     return TTC_OK;
 }
@@ -1122,7 +1139,7 @@ ttc_status ttc_linear(ttc_ctx* c, const ttc_linear_desc* d, const void* d_x, con
         return c->fail(TTC_ERR_ARG, "linear: res_pitch must be at least cout");
     if (d->rows == 0) return TTC_OK;
     const bool narrow = narrow_fwd(d);
-    const int sp = narrow ? 1 : gemm_splits(d->rows, d->cout, d->cin, LEAST_K);
+    const int sp = narrow ? 1 : gemm_splits(d->rows, d->cout, d->cin, LEAST_K, dtype_bytes(d->dtype));
     if (!d_x || !d_w || !d_y || (sp > 1 && !d_ws)) return c->fail(TTC_ERR_ARG, "linear: null pointer");
     if (sp > 1 && ws_bytes < (size_t)sp * d->rows * d->cout * sizeof(float))
         return c->fail(TTC_ERR_ARG, "linear: workspace smaller than ttc_linear_workspace asks for");
@@ -1186,7 +1203,7 @@ ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void*
             GemmArgs a = fwd_args(d, d_x, d_w);
             GemmArgs zf = a;
             zf.fwd = 1; zf.act = TTC_ACT_NONE; zf.alpha = 1.0f; zf.bias = d_bias; zf.C = nullptr; zf.preact = (float*)ws;
-            gemm_launch<T, true, false>(zf, gemm_splits(d->rows, d->cout, d->cin, LEAST_K), (float*)(ws + w.part), s);
+            gemm_launch<T, true, false>(zf, gemm_splits(d->rows, d->cout, d->cin, LEAST_K, dtype_bytes(d->dtype)), (float*)(ws + w.part), s);
             z = (const float*)ws;
         }
         const T* dz = act ? (const T*)(ws + w.dz) : (const T*)d_dy;     // without an activation dz is dy itself; the scale is in the epilogues either way
