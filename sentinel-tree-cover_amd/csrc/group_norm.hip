@@ -691,6 +691,7 @@ ttc_status ttc_group_norm(ttc_ctx* c, const ttc_group_norm_desc* d, const void* 
     NormPlan p = norm_plan(d, false);
     NormArgs& a = p.a;
     if (!d_x || !d_y || (p.ws.total && !d_ws)) return c->fail(TTC_ERR_ARG, "group_norm: null pointer");
+    if ((uintptr_t)d_ws % 16) return c->fail(TTC_ERR_ARG, "group_norm: the workspace must be 16-byte aligned");
     if (ws_bytes < p.ws.total) return c->fail(TTC_ERR_ARG, "group_norm: workspace smaller than ttc_group_norm_workspace asks for");
     a.x = d_x; a.gamma = d_gamma; a.beta = d_beta; a.y = d_y; a.stats = d_stats; a.part = (double*)d_ws;
     DeviceGuard dev(c->device);
@@ -736,6 +737,7 @@ ttc_status ttc_group_norm_backward(ttc_ctx* c, const ttc_group_norm_desc* d, con
     if (!empty) {
         p = norm_plan(d, true);
         if (!d_x || !d_dy || !d_stats || !d_ws) return c->fail(TTC_ERR_ARG, "group_norm_backward: null pointer");
+        if ((uintptr_t)d_ws % 16) return c->fail(TTC_ERR_ARG, "group_norm_backward: the workspace must be 16-byte aligned");
         if (ws_bytes < p.ws.total) return c->fail(TTC_ERR_ARG, "group_norm_backward: workspace smaller than ttc_group_norm_workspace asks for");
     } else {
         p.a.C = d->channels;

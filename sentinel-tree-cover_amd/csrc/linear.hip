@@ -474,6 +474,70 @@ __global__ __launch_bounds__(NT) void k_join(GemmArgs a, const float* __restrict
     }
 }
 
+// ---- a few rows: the weights pass once, straight through the vector ALU ------------------------------------------------------------------
+// y of MR rows is bound by reading w (and, for one row, by the launch).  A lane owns 16 bytes of columns and every KL-th row of w, so a workgroup
+// covers `lanes` x 16 bytes of columns and the whole contracted index: no partials in memory, one launch.  Narrow column runs give enough
+// workgroups; those that share a cache line of w run on one XCD and meet in its L2.  The KL partial sums of a column are a tree in LDS.
+template <class T, int MR>
+__global__ __launch_bounds__(NT) void k_few(GemmArgs a, int lanes) {
+    constexpr int V = VE<T>;
+    __shared__ float red[NT * MR * V];
+    const int total = gridDim.x, bid = blockIdx.x, xcd = bid & 7, per = total >> 3, rem = total & 7;
+    const int tile = xcd * per + min(xcd, rem) + (bid >> 3);
+    const int tid = threadIdx.x, cl = tid & (lanes - 1), kl = tid / lanes, KL = NT / lanes;
+    const int col = (tile * lanes + cl) * V, left = a.N - col;
+    float acc[MR][V];
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[m][i] = 0.0f;
+    if (left > 0) {
+        const T* w = (const T*)a.B + col;
+        const T* x = (const T*)a.A;
+        const int K = (int)a.K;
+        if (left >= V) {
+#pragma unroll 8
+            for (int k = kl; k < K; k += KL) {
+                float wv[V];
+                load_vec<T, V>(w + (long)k * a.ldb, wv);
+#pragma unroll
+                for (int m = 0; m < MR; ++m) {
+                    const float xv = (float)x[min((long)m, a.M - 1) * a.lda + k];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc[m][i] += xv * wv[i];
+                }
+            }
+        } else {
+            for (int k = kl; k < K; k += KL)
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (i < left) {
+                        const float wv = (float)w[(long)k * a.ldb + i];
+#pragma unroll
+                        for (int m = 0; m < MR; ++m) acc[m][i] += (float)x[min((long)m, a.M - 1) * a.lda + k] * wv;
+                    }
+        }
+    }
+    const int width = lanes * MR * V;                        // [kl][row][column]
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int i = 0; i < V; ++i) red[kl * width + (m * lanes + cl) * V + i] = acc[m][i];
+    for (int half = KL / 2; half; half /= 2) {
+        __syncthreads();
+        for (int i = tid; i < half * width; i += NT) red[i] += red[half * width + i];
+    }
+    __syncthreads();
+    for (int i = tid; i < lanes * MR; i += NT) {
+        const int m = i / lanes, c = (tile * lanes + (i & (lanes - 1))) * V;
+        if (m >= a.M || c >= a.N) continue;
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = red[i * V + j];
+        emit<T, V>(a, m, c, a.N - c, v);
+    }
+}
+
 // ---- narrow products: the weights stay in LDS ------------------------------------------------------------------------------------------------
 // x w for cin <= 16-byte steps KS of the contracted index, cout <= 16 FN: bound by the rows' bytes.  A wave takes 16 rows at a time and needs no
 // other wave: x goes from memory straight into fragments (a lane's 16 bytes ARE the fragment), the next rows' while this row's products run, and
@@ -707,9 +771,12 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
             x[h].trim(a.K, q);
             d[h].trim(a.N, q);
             const int left = (int)max(min(a.M - (g * RW + h * 16), 16L), 0L);
-            if (r >= left)
+            if (r >= left) {                                 // no row there: nothing of what was read instead may reach dw (0 x inf is not 0)
 #pragma unroll
                 for (int p = 0; p < NS; ++p) d[h].v[p] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int s = 0; s < KS; ++s) x[h].v[s] = make_uint4(0, 0, 0, 0);
+            }
             Frag dz[NS];
             if (a.act == TTC_ACT_NONE) {
 #pragma unroll
@@ -966,6 +1033,7 @@ void gemm_launch(GemmArgs a, int splits, float* ws, hipStream_t s) {
                 if (splits > 1) join_launch<T>(j, ws, a.M * a.N, splits, 0, nullptr, s);
                 return;
             }
+            (void)hipGetLastError();                         // the LDS size was refused: the smaller tiles do it
         }
     }
     const int bn = bn_of(a.N), bm = bm_of(a.M, a.N);
@@ -1014,6 +1082,20 @@ void narrow_launch(const GemmArgs& a, hipStream_t s) {
     else if (ks <= 2) narrow_launch_k<T, 2>(a, s);
     else if (ks <= 4) narrow_launch_k<T, 4>(a, s);
     else narrow_launch_k<T, 8>(a, s);
+}
+// a few rows that are not narrow: k_few.  1024 -> 4096, us by k_few / by split tiles: bf16 1 row 5.0 / 9.2, 4 rows 7.2 / 8.1, 8 rows 10.0 / 8.1;
+// fp32 8 rows 8.8 / 13.5 (half the columns a lane, so half the sums a row costs it)
+bool few_rows(const ttc_linear_desc* d) { return d->rows <= (d->dtype == TTC_DT_F32 ? 8 : 4) && !narrow_fwd(d); }
+template <class T>
+void few_launch(const GemmArgs& a, hipStream_t s) {
+    const long runs = (a.N + VE<T> - 1) / VE<T>;             // 16-byte column runs
+    int lanes = 2;                                           // 32 bytes of columns a workgroup, wider where that makes more than 1024 of them
+    while (lanes < 64 && runs / lanes > 1024) lanes *= 2;
+    const dim3 grid((unsigned)((runs + lanes - 1) / lanes));
+    if (a.M <= 1) hipLaunchKernelGGL((k_few<T, 1>), grid, dim3(NT), 0, s, a, lanes);
+    else if (a.M <= 2) hipLaunchKernelGGL((k_few<T, 2>), grid, dim3(NT), 0, s, a, lanes);
+    else if (a.M <= 4) hipLaunchKernelGGL((k_few<T, 4>), grid, dim3(NT), 0, s, a, lanes);
+    else if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((k_few<T, 8>), grid, dim3(NT), 0, s, a, lanes);
 }
 int narrow_bwd_blocks(const ttc_linear_desc* d) {
     const long rw = d->dtype == TTC_DT_F32 ? 64 : 128;        // rows of a workgroup's step
@@ -1122,7 +1204,7 @@ ttc_status ttc_linear_workspace(const ttc_linear_desc* d, int32_t backward, size
     if (linear_check(d)) return TTC_ERR_ARG;
     if (d->rows == 0) return TTC_OK;
     if (backward) { *bytes = linear_ws(d, backward == TTC_LINEAR_HAVE_PREACT).total; return TTC_OK; }
-    const int sp = narrow_fwd(d) ? 1 : gemm_splits(d->rows, d->cout, d->cin, LEAST_K, dtype_bytes(d->dtype));
+    const int sp = narrow_fwd(d) || few_rows(d) ? 1 : gemm_splits(d->rows, d->cout, d->cin, LEAST_K, dtype_bytes(d->dtype));
     if (sp > 1) *bytes = (size_t)sp * d->rows * d->cout * sizeof(float);
     return TTC_OK;
 }
@@ -1138,9 +1220,10 @@ ttc_status ttc_linear(ttc_ctx* c, const ttc_linear_desc* d, const void* d_x, con
     if (d_residual && ((d->rows > 1 && d->res_pitch < d->cout) || d->res_pitch > (1L << 30)))
         return c->fail(TTC_ERR_ARG, "linear: res_pitch must be at least cout");
     if (d->rows == 0) return TTC_OK;
-    const bool narrow = narrow_fwd(d);
-    const int sp = narrow ? 1 : gemm_splits(d->rows, d->cout, d->cin, LEAST_K, dtype_bytes(d->dtype));
+    const bool narrow = narrow_fwd(d), few = few_rows(d);
+    const int sp = narrow || few ? 1 : gemm_splits(d->rows, d->cout, d->cin, LEAST_K, dtype_bytes(d->dtype));
     if (!d_x || !d_w || !d_y || (sp > 1 && !d_ws)) return c->fail(TTC_ERR_ARG, "linear: null pointer");
+    if (sp > 1 && (uintptr_t)d_ws % 16) return c->fail(TTC_ERR_ARG, "linear: the workspace must be 16-byte aligned");
     if (sp > 1 && ws_bytes < (size_t)sp * d->rows * d->cout * sizeof(float))
         return c->fail(TTC_ERR_ARG, "linear: workspace smaller than ttc_linear_workspace asks for");
     DeviceGuard dev(c->device);
@@ -1153,6 +1236,7 @@ ttc_status ttc_linear(ttc_ctx* c, const ttc_linear_desc* d, const void* d_x, con
     const ttc_status st = with_dtype(d->dtype, [&](auto tag) {
         using T = decltype(tag);
         if (narrow) narrow_launch<T>(a, s);
+        else if (few) few_launch<T>(a, s);
         else gemm_launch<T, true, false>(a, sp, (float*)d_ws, s);
         return TTC_OK;
     });
@@ -1171,6 +1255,7 @@ ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void*
     if (d->rows > 0) {
         w = linear_ws(d, !again);
         if (!d_dy || ((d_dw || again) && !d_x) || ((d_dx || again) && !d_w) || !d_ws) return c->fail(TTC_ERR_ARG, "linear_backward: null pointer");
+        if ((uintptr_t)d_ws % 16) return c->fail(TTC_ERR_ARG, "linear_backward: the workspace must be 16-byte aligned");
         if (ws_bytes < w.total) return c->fail(TTC_ERR_ARG, "linear_backward: workspace smaller than ttc_linear_workspace asks for");
     }
     DeviceGuard dev(c->device);
