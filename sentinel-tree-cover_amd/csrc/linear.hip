@@ -350,83 +350,87 @@ __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
     store_tile<T>(a, acc, m0 + wm * WM, n0 + wn * WN, lane);
 }
 
-// ---- the wide tile kernel: 16-bit operands, 256 x 256 -------------------------------------------------------------------------------------
-// One workgroup of 8 waves per CU (2 x 4, 128 x 64 outputs each: 24 KB of LDS fragments per wave and step against 64 matrix instructions, 3/4 of the
-// LDS rate), two 64 KB stages.  Tiles go from memory to LDS without passing registers, 16 bytes a lane; the swizzle is in which piece of its row a
-// lane fetches.  A stage is fetched while the other is multiplied; one barrier a step.  Rows and columns past the array fetch the last ones (not stored);
-// the contracted range is a multiple of 64 and every row 16-byte aligned: other calls take k_gemm.
+// ---- the wide tile kernel: 256 x 256 (16-bit) or 256 x 128 ------------------------------------------------------------------------------------
+// One workgroup of 8 waves per CU, two stages in LDS (16-bit 256 x 256: a wave's 128 x 64 outputs read 24 KB of LDS fragments per step against 64 matrix
+// instructions, 3/4 of the LDS rate; 8192 x 4096 x 4096 bf16 measured 1.1 - 1.35 PFLOP/s, the library's product 1.3).  Tiles go from memory to LDS
+// without passing registers, 16 bytes a lane; the swizzle is in which piece of its row a lane fetches.  A stage is fetched while the other is
+// multiplied; one barrier a step.  Rows and columns past the array fetch the last ones (not stored); the contracted range is whole steps and every row
+// 16-byte aligned: other calls take k_gemm.
 // The copy is written out because the compiler, which cannot tell the stages apart, waits for every copy in flight before each LDS read.  It has no
 // register result; the wait for it is the explicit one in front of the barrier.
-template <class T, bool KC>
+template <class T, bool KC, int BF>
 struct WideTile {
-    unsigned off[4];                               // a lane's pieces, bytes from the step's base
+    static constexpr int CNT = BF / 64, PR = BF / VE<T>, PG = sizeof(T);     // pieces a lane, pieces of a row as stored (FC), pieces of a swizzled run
+    unsigned off[CNT];                             // a lane's pieces, bytes from the step's base
     __device__ __forceinline__ void init(long ld, long f0, long F, int wave, int lane) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < CNT; ++i) {
             const int id = (i * 8 + wave) * 64 + lane;
             if (KC) {
                 const int row = id >> 3, ch = (id & 7) ^ ((row ^ (row >> 3)) & 7);
-                off[i] = (unsigned)min((long)row, F - 1 - f0) * (unsigned)(ld * 2) + ch * 16;
+                off[i] = (unsigned)min((long)row, F - 1 - f0) * (unsigned)(ld * (long)sizeof(T)) + ch * 16;
             } else {
-                const int k = id >> 5, c = id & 31, sw = (k & 3) | ((k >> 1) & 4);
-                off[i] = (unsigned)k * (unsigned)(ld * 2) + (unsigned)min((long)(((c >> 1) ^ sw) * 16 + (c & 1) * 8), F - 8 - f0) * 2;
+                const int k = id / PR, c = id % PR, sw = sizeof(T) == 2 ? (k & 3) | ((k >> 1) & 4) : (k >> 2) & 3;
+                const int col = ((c / PG) ^ (sw & (BF / 16 - 1))) * 16 + (c % PG) * VE<T>;
+                off[i] = (unsigned)k * (unsigned)(ld * (long)sizeof(T)) + (unsigned)min((long)col, F - VE<T> - f0) * (unsigned)sizeof(T);
             }
         }
     }
     __device__ __forceinline__ void fetch(const T* p, long ld, long f0, long k, unsigned lds, int wave) const {
         const T* base = KC ? p + f0 * ld + k : p + k * ld + f0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < CNT; ++i)
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds + (i * 8 + wave) * 1024u), "v"(off[i]), "s"(base) : "memory", "m0");
     }
 };
-template <class T, bool AKC, bool BKC>
+constexpr int WIDE_LDS(int bn) { return 2 * (256 + bn) * 128; }
+template <class T, bool AKC, bool BKC, int BN>
 __global__ __launch_bounds__(512) void k_gemm_wide(GemmArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char wide_lds[];      // A0 A1 B0 B1, 32 KB each
-    constexpr int TB = 256 * 128;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
+    extern __shared__ __attribute__((aligned(16))) char wide_lds[];      // A0 A1 B0 B1
+    constexpr int TA = 256 * 128, TB = BN * 128, WGN = BN / 64, WM = 256 / (8 / WGN), FM = WM / 16;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WGN, wn = wave % WGN;
     const int total = a.mt * a.nt, bid = blockIdx.x, xcd = bid & 7, per = total >> 3, rem = total & 7;
     const int tile = xcd * per + min(xcd, rem) + (bid >> 3);
     const long m0 = (long)(tile / a.nt) * 256;
-    const int n0 = (tile % a.nt) * 256;
+    const int n0 = (tile % a.nt) * BN;
     const long k0 = blockIdx.y * a.k_per, k1 = min(k0 + a.k_per, a.K);
     const T* A = (const T*)a.A;
     const T* B = (const T*)a.B;
-    f32x4 acc[4][8];
+    f32x4 acc[4][FM];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)wide_lds;
-    WideTile<T, AKC> ta;
-    WideTile<T, BKC> tb;
+    WideTile<T, AKC, 256> ta;
+    WideTile<T, BKC, BN> tb;
     ta.init(a.lda, m0, a.M, wave, lane);
     tb.init(a.ldb, n0, a.N, wave, lane);
     ta.fetch(A, a.lda, m0, k0, lds0, wave);
-    tb.fetch(B, a.ldb, n0, k0, lds0 + 2 * TB, wave);
+    tb.fetch(B, a.ldb, n0, k0, lds0 + 2 * TA, wave);
     __builtin_amdgcn_s_waitcnt(0x0f70);            // vmcnt(0): this wave's pieces have landed; the barrier makes that everyone's
     __syncthreads();
     int cur = 0;
-    for (long k = k0; k < k1; k += 64, cur ^= 1) {
-        if (k + 64 < k1) {                         // the other stage was last read before the barrier
-            ta.fetch(A, a.lda, m0, k + 64, lds0 + (cur ^ 1) * TB, wave);
-            tb.fetch(B, a.ldb, n0, k + 64, lds0 + (2 + (cur ^ 1)) * TB, wave);
+    for (long k = k0; k < k1; k += BKE<T>, cur ^= 1) {
+        if (k + BKE<T> < k1) {                     // the other stage was last read before the barrier
+            ta.fetch(A, a.lda, m0, k + BKE<T>, lds0 + (cur ^ 1) * TA, wave);
+            tb.fetch(B, a.ldb, n0, k + BKE<T>, lds0 + 2 * TA + (cur ^ 1) * TB, wave);
         }
-        const char* la = wide_lds + cur * TB;
-        const char* lb = wide_lds + (2 + cur) * TB;
+        const char* la = wide_lds + cur * TA;
+        const char* lb = wide_lds + 2 * TA + cur * TB;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            typename Mma<T>::Frag fa[8], fb[4];
+            typename Mma<T>::Frag fa[FM], fb[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fb[i] = frag<T, BKC, 256, true>(lb, wn * 64, i, ks, lane);
+            for (int i = 0; i < 4; ++i) fb[i] = frag<T, BKC, BN, true>(lb, wn * 64, i, ks, lane);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) fa[j] = frag<T, AKC, 256, false>(la, wm * 128, j, ks, lane);
+            for (int j = 0; j < FM; ++j) fa[j] = frag<T, AKC, 256, false>(la, wm * WM, j, ks, lane);
             mma_block<T>(acc, fb, fa);
         }
         __builtin_amdgcn_s_waitcnt(0x0f70);
         __syncthreads();
     }
-    store_tile<T>(a, acc, m0 + wm * 128, n0 + wn * 64, lane);
+    store_tile<T>(a, acc, m0 + wm * WM, n0 + wn * 64, lane);
 }
 
 // ---- joining the splits of the contracted index: C = epilogue(sum of the partials), 4 columns a thread, L lanes over the splits -------------------
@@ -988,16 +992,25 @@ __global__ void k_fill0(T* p, long n) {
 int bn_of(long N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }       // column tile: narrower only where the wide one would be mostly padding
 // row tile: 64 rows where 128 would leave CUs without a tile (5003 x 93 -> 177: 8.7 -> 6.2 us; but 8192 x 1024 -> 4096: 133 -> 159, twice the reads of w)
 int bm_of(long M, long N) { return bn_of(N) == 128 && ((M + 127) / 128) * ((N + 127) / 128) < 256 ? 64 : 128; }
-// the 256 x 256 kernel: where its tiles fill the CUs, or do with the contracted index split into runs of at least 1024
-constexpr long WIDE_PITCH = 1L << 22;                         // 256 rows of them fit a 32-bit byte offset
-long wide_tiles(long M, long N) { return ((M + 255) / 256) * ((N + 255) / 256); }
-bool wide_ok(long M, long N, long K) { return K % 64 == 0 && M >= 256 && N >= 256 && wide_tiles(M, N) * std::max<long>(1, K / 1024) >= 192; }
+// the wide kernel's columns (0: not for this product): 256 for 16-bit types where its tiles fill the CUs, or do with the contracted index split into
+// runs of at least 1024; 128 where those fill most of them
+constexpr long WIDE_PITCH = 1L << 21;                         // 256 rows of them fit a 32-bit byte offset
+#ifndef W128
+#define W128 192
+#endif
+long wide_tiles(long M, long N, long bn) { return ((M + 255) / 256) * ((N + bn - 1) / bn); }
+int wide_cols(long M, long N, long K, int bytes) {
+    if (K % (128 / bytes) || M < 256 || N < 128) return 0;
+    const long runs = std::max<long>(1, K / 1024);
+    if (bytes == 2 && N >= 256 && wide_tiles(M, N, 256) * runs >= 192) return 256;
+    return wide_tiles(M, N, 128) >= W128 ? 128 : 0;
+}
 // how many ways the contracted index is split: one where the tiles fill the CUs; else so that one workgroup per CU runs, two where the index is long
 // (4096 x 1024 -> 1024 bf16: y 23 us with one, 34 with two; dw of 65536 x 512 -> 256: 76 us with one, 56 with two), each with at least `least` of it,
 // and the partials stay under 64 MB
 int gemm_splits(long M, long N, long K, long least, int bytes) {
     const long fit = std::max<long>(1, (64L << 20) / (M * N * 4));
-    if (bytes == 2 && wide_ok(M, N, K)) return (int)std::max<long>(1, std::min<long>({256 / wide_tiles(M, N), K / 1024, fit}));
+    if (const int wn = wide_cols(M, N, K, bytes)) return (int)std::max<long>(1, std::min<long>({256 / wide_tiles(M, N, wn), K / 1024, fit}));
     const long bm = bm_of(M, N), tiles = ((M + bm - 1) / bm) * ((N + bn_of(N) - 1) / bn_of(N));
     return (int)std::max<long>(1, std::min<long>({(K > 4096 ? 512 : 256) / tiles, K / least, fit}));
 }
@@ -1022,19 +1035,24 @@ void gemm_launch(GemmArgs a, int splits, float* ws, hipStream_t s) {
         splits = (int)((a.K + a.k_per - 1) / a.k_per);
     }
     if (splits > 1) { a.C = ws; a.partial = 1; }
-    if constexpr (sizeof(T) == 2) {
-        if (wide_ok(a.M, a.N, a.K) && a.lda % 8 == 0 && a.ldb % 8 == 0 && a.lda <= WIDE_PITCH && a.ldb <= WIDE_PITCH && (uintptr_t)a.A % 16 == 0 && (uintptr_t)a.B % 16 == 0 && (AKC || a.M % 8 == 0)
-            && (BKC || a.N % 8 == 0)) {
-            static LdsConfig cfg;
-            if (cfg.ensure(k_gemm_wide<T, AKC, BKC>, 4 * 256 * 128) == hipSuccess) {
-                a.mt = (int)((a.M + 255) / 256);
-                a.nt = (a.N + 255) / 256;
-                hipLaunchKernelGGL((k_gemm_wide<T, AKC, BKC>), dim3((unsigned)(a.mt * a.nt), splits), dim3(512), 4 * 256 * 128, s, a);
-                if (splits > 1) join_launch<T>(j, ws, a.M * a.N, splits, 0, nullptr, s);
-                return;
+    if (const int wn = wide_cols(a.M, a.N, a.K, sizeof(T));
+        wn && a.lda % VE<T> == 0 && a.ldb % VE<T> == 0 && a.lda <= WIDE_PITCH && a.ldb <= WIDE_PITCH && (uintptr_t)a.A % 16 == 0 && (uintptr_t)a.B % 16 == 0
+        && (AKC || a.M % VE<T> == 0) && (BKC || a.N % VE<T> == 0)) {
+        auto go = [&](auto fn, LdsConfig& cfg) {
+            if (cfg.ensure(fn, WIDE_LDS(wn)) != hipSuccess) {
+                (void)hipGetLastError();                     // the LDS size was refused: the smaller tiles do it
+                return false;
             }
-            (void)hipGetLastError();                         // the LDS size was refused: the smaller tiles do it
-        }
+            a.mt = (int)((a.M + 255) / 256);
+            a.nt = (a.N + wn - 1) / wn;
+            hipLaunchKernelGGL(fn, dim3((unsigned)(a.mt * a.nt), splits), dim3(512), WIDE_LDS(wn), s, a);
+            if (splits > 1) join_launch<T>(j, ws, a.M * a.N, splits, 0, nullptr, s);
+            return true;
+        };
+        static LdsConfig c128, c256;
+        if (wn == 128 && go(k_gemm_wide<T, AKC, BKC, 128>, c128)) return;
+        if constexpr (sizeof(T) == 2)
+            if (wn == 256 && go(k_gemm_wide<T, AKC, BKC, 256>, c256)) return;
     }
     const int bn = bn_of(a.N), bm = bm_of(a.M, a.N);
     a.mt = (int)((a.M + bm - 1) / bm);

@@ -260,10 +260,10 @@ def test_linear(ctx, dtype, shape):
                  randn((m, n), dt, 150 + i) if i % 2 else None, act, scale=(1.0, 0.1)[i // 2 % 2], dy=randn((m, n), dt, 200 + i))
 
 
-@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
-@pytest.mark.parametrize("shape", [(3333, 128, 3848), (3333, 3848, 128), (192, 3336, 3848), (1000, 12352, 1000), (3584, 64, 4096)], ids=str)
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(9999, 64, 640), (9999, 640, 64), (64, 9996, 640), (3333, 128, 3848), (3333, 3848, 128), (192, 3336, 3848), (1000, 12352, 1000), (3584, 64, 4096)], ids=str)
 def test_linear_wide(ctx, dtype, shape):
-    """16-bit products of many 256 x 256 tiles, ragged at the far edges: in y, in dx, in dw, with the contracted index split; the strided and the
+    """products of many 256 x 256 or 256 x 128 tiles, ragged at the far edges: in y, in dx, in dw, with the contracted index split; the strided and the
     misaligned call give the aligned call's bits or stay within the bounds"""
     m, k, n = shape
     dt = DT[dtype]
