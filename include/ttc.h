@@ -446,7 +446,8 @@ ttc_status ttc_s1_to_db(ttc_ctx* ctx, const uint16_t* d_u16, int32_t T, int32_t 
  *                   (TF layout [1, 1, cin, cout]); the graph's 1x1 sigmoid head (src/train/train-model.py:226-231) is
  *                   linear(late, head/kernel, head/bias, sigmoid)
  * Arrays are fp32, fp16 or bf16 (one type per call); gamma, beta, bias, the statistics and the gradients of gamma, beta and bias are always
- * float32.  Sums and statistics are held in 32 bits or more, results are rounded once; no atomics: two runs give the same bits.
+ * float32.  Sums and statistics are held in 32 bits or more, results are rounded once (and dz of ttc_linear_backward once to the arrays' type,
+ * as operand of the two matrix products); no atomics: two runs give the same bits.
  * Nothing here uses the context's workspace, weights or window geometry: the caller passes the scratch memory the *_workspace query
  * names (16-byte aligned), so calls on several streams and calls captured into several graphs do not share any.  No call allocates, synchronises or
  * copies; all of them can be captured into a graph.  Rows need unit channel stride and may be a slice of wider rows; a row may start at any
@@ -491,8 +492,9 @@ int32_t    ttc_linear_wants_preact(const ttc_linear_desc* desc);
 ttc_status ttc_linear(ttc_ctx* ctx, const ttc_linear_desc* desc, const void* d_x, const void* d_w, const float* d_bias, const void* d_residual,
                       void* d_y, float* d_preact, void* d_ws, size_t ws_bytes, void* stream);
 /* gradients of ttc_linear: with dz = scale * dy * act'(x w + bias), d_dx [rows, cin] = dz w^T, d_dw [cin, cout] = x^T dz (0 for rows = 0),
- * d_dbias [cout] float32 = column sums of dz; each may be NULL.  The residual's gradient is dy.  With an activation the argument of act' comes from
- * d_preact, or, where that is NULL, from x, w and d_bias again (the d_bias of the forward call; not read otherwise). */
+ * d_dbias [cout] float32 = column sums of dz; each of these three may be NULL, d_dy, d_x and d_w may not.  The residual's gradient is dy.
+ * With an activation the argument of act' comes from d_preact, or, where that is NULL, from x, w and d_bias again (the d_bias of the forward
+ * call; not read otherwise). */
 ttc_status ttc_linear_backward(ttc_ctx* ctx, const ttc_linear_desc* desc, const void* d_dy, const void* d_x, const void* d_w, const float* d_bias,
                                const float* d_preact, void* d_dx, void* d_dw, float* d_dbias, void* d_ws, size_t ws_bytes, void* stream);
 

@@ -62,6 +62,7 @@ __device__ __forceinline__ void mean_rstd(double s, double q, double count, floa
 }
 
 // ---- forward, pass 1: partial sums per (sample, slot, group) ------------------------------------------------------------------------
+// Bound by reading x: 36 x 172 x 172 x 64 fp32 (273 MB) 66 us = 4.1 TB/s, bf16 22 us (6 TB/s, from the last-level cache).
 // UNI: a thread's V channels share a group, so one pair of sums (about the thread's first element) serves them all
 template <class T, int V, bool UNI>
 __global__ __launch_bounds__(NT) void k_gn_sums(NormArgs a) {
@@ -178,6 +179,7 @@ struct Chan {
 };
 
 // ---- forward, pass 2: y = act(gamma xh + beta) ----------------------------------------------------------------------------------------
+// Bound by memory: 36 x 172 x 172 x 64 fp32 swish 88 us = 6.2 TB/s read and written, bf16 49 us = 5.6; 36 x 84 x 84 x 128 bf16 sigmoid 27 us.
 template <class T, int V, bool UNI>
 __global__ __launch_bounds__(NT) void k_gn_apply(NormArgs a) {
     extern __shared__ float sg[];                  // [G][2]
@@ -227,6 +229,7 @@ __global__ __launch_bounds__(NT) void k_gn_apply(NormArgs a) {
 }
 
 // ---- backward, pass 1: sum dz, sum dz xh per (sample, slot, channel) -----------------------------------------------------------------
+// 36 x 172 x 172 x 64 bf16 swish: 59 us = 4.6 TB/s of x and dy; the slope costs about 36 us of vector ALU under it.
 template <class T, int V, bool UNI>
 __global__ __launch_bounds__(NT) void k_gn_bwd_sums(NormArgs a) {
     extern __shared__ float sf[];                  // [rpb][cols * V][2]
@@ -355,6 +358,7 @@ struct ChanBwd : Chan<V, UNI> {
 };
 
 // ---- backward, pass 2: dx, and in blocks of their own (the last of every sample's row) the parameters' gradients --------------------------
+// 36 x 172 x 172 x 64 bf16 swish: 77 us = 5.3 TB/s.
 template <class T, int V, bool UNI>
 __global__ __launch_bounds__(NT) void k_gn_bwd_apply(NormArgs a) {
     if ((int)blockIdx.x == a.splits) {
@@ -398,7 +402,8 @@ __global__ __launch_bounds__(NT) void k_gn_bwd_apply(NormArgs a) {
 
 // ---- one launch: a workgroup holds whole groups of a sample ------------------------------------------------------------------------------
 // blockIdx.x = slab of a.cols * V channels (whole groups, V divides channels / groups), blockIdx.y = sample; RU vectors a thread stay in registers
-// as stored.
+// as stored.  14 x 14 x 64 fp32: 4.7 us against 4.2 + 4.7 by two launches; 32 x 28 x 28 x 64 fp32 6.5 against 5.5 + 6.4, backward 11 + 4 against 23;
+// 5 x 61 x 47 x 40 fp16 10.5 against 14 (with 8 vectors a thread: 14.6, too few workgroups share the chip).
 template <class T, int V>
 struct Held {
     static constexpr int W = V * sizeof(T) >= 4 ? V * sizeof(T) / 4 : 1;
@@ -483,7 +488,8 @@ __global__ __launch_bounds__(RT) void k_gn_resident(NormArgs a) {
     }
 }
 
-// the same for the backward pass: x is held, dy read again for dx (holding both spills: its second read comes from the L2); the sums of a channel over the rows are a 32-bit tree in LDS.  direct: one sample, so its sums ARE the parameters'
+// the same for the backward pass: x is held, dy read again for dx (holding both spills: its second read comes from the L2); the sums of a channel over
+// the rows are a 32-bit tree in LDS.  direct: one sample, so its sums ARE the parameters'
 // gradients
 template <class T, int V>
 __global__ __launch_bounds__(RT) void k_gn_resident_bwd(NormArgs a, int direct) {

@@ -49,7 +49,7 @@ __device__ __forceinline__ float normal_tail(float z, float* e) {
     const float az = fabsf(z), t = __builtin_amdgcn_rcpf(1.0f + (0.356f * 0.70710678f) * az);
     const float p = 0.100425743f + t * (0.100426443f + t * (0.094032362f + t * (0.081815816f + t * (0.0595245f + t * (0.061009083f
                     + t * (-0.027474117f + t * (0.08918602f + t * (-0.078777514f + t * 0.01983167f))))))));
-    *e = __expf(-0.5f * z * z);
+    *e = __builtin_amdgcn_exp2f(-0.72134752f * (z * z));        // log2(e) / 2
     return t * p * *e;
 }
 

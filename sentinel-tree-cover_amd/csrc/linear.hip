@@ -4,14 +4,19 @@
 //   z = x w + b,  y = residual + scale act(z)            x [m, k], w [k, n] (TF layout: the output channel is contiguous)
 //   dz = scale dy act'(z);  dx = dz w^T;  dw = x^T dz;  db = column sums of dz
 //
-// All three products run the one tile kernel k_gemm: C[i, j] = sum_c A(i, c) B(c, j), where each operand is stored either with the contracted index
-// contiguous ("KC": x and dz in dx, w in dx) or with its free index contiguous ("FC": w in y, x and dz in dw).
+// A product is C[i, j] = sum_c A(i, c) B(c, j), where each operand is stored either with the contracted index contiguous ("KC": x and dz in dx, w in dx) or
+// with its free index contiguous ("FC": w in y, x and dz in dw).  By size (host code at the end):
+//   k_narrow, k_narrow_bwd   up to 128 columns, weights in LDS: bound by the rows' bytes; the backward pass in one pass over the rows
+//   k_few                    a few rows: bound by reading w
+//   k_gemm_wide              many 256 x 256 / 256 x 128 tiles of aligned rows: bound by the matrix cores
+//   k_gemm                   everything else; with few tiles the contracted index is split and k_join adds the parts
+// All but k_few share the fragments:
 //  - KC tiles lie in LDS as rows of 128 bytes; a lane reads 16 bytes = its 8 (16-bit) or 4 (fp32) values of the contracted index.
 //  - FC tiles lie in LDS as stored; 16-bit fragments come through the transposing LDS read (ds_read_tr16_b64), fp32 ones through single words.
 //  - the contracted index may be permuted freely as long as both operands agree: that is what makes the 16-byte KC read fit the fp32 instruction.
 //  - the matrix instruction gets B's fragment first, so a lane ends up with consecutive OUTPUT CHANNELS of one row (8 for 16-bit types: the rows of
 //    fragment pairs are interleaved) and stores 16 bytes at a time.
-// LDS slots are XOR-swizzled so that no fragment read has more than a two-way bank conflict.
+//  - LDS slots are XOR-swizzled against bank conflicts.
 #include <algorithm>
 
 #include "layers_common.h"
@@ -49,12 +54,7 @@ template <> struct Mma<bf16> {
     static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mma<float> {
-    typedef f32x4 Frag;             // 4 values of the contracted index = 4 instructions of 4
-    static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-        return c;
-    }
+    typedef f32x4 Frag;             // 4 values of the contracted index = 4 instructions of 4 (mma_block)
 };
 
 // acc[i][j] += b[i] a[j]: the instructions of one accumulator are as far apart as there are accumulators (fp32: four per pair; back to back each waited
@@ -189,7 +189,7 @@ __device__ __forceinline__ typename Mma<T>::Frag frag(const char* lds, int base,
     }
 }
 
-// V consecutive columns of one row, `left` of them exist: the forward epilogue on x w, with the bias and the residual in hand
+// V consecutive columns of one row, `left` of them exist
 template <class T, int V>
 __device__ __forceinline__ void store_part(T* p, int left, const float (&v)[V]) {
     if (left >= V) { store_vec<T, V>(p, v); return; }
@@ -252,54 +252,68 @@ __device__ __forceinline__ void emit(const GemmArgs& a, long row, int col, int l
     }
 }
 
-// a wave's accumulators (FN fragments of columns, FM of rows) from row m0, column n0.  Columns outermost: a lane's bias is loaded once for all its rows.
-template <class T, int FN, int FM>
-__device__ __forceinline__ void store_tile(const GemmArgs& a, f32x4 (&acc)[FN][FM], long m0, int n0, int lane) {
-    const int r = lane & 15, q = lane >> 4;
-    constexpr int V = VE<T>, NV = FN * 16 / (4 * V), NR = NV == 1 ? 1 : 2;      // columns a lane stores at once, such runs of a wave, rows of each
-    const int hi = NR == 1 ? 0 : r >> 3, r0 = NR == 1 ? r : r & 7;
+// A wave's accumulators (FN fragments of columns, FM of rows) from row m0, column n0, through its own piece of LDS (free after the last step), JC row
+// fragments at a time.  There a lane finds whole 16-byte runs of a row, its columns (and its bias) the same for every row, and 64 lanes whole lines: no
+// trade.  And the epilogue is a LOOP: unrolled over the accumulators, with its five activations, it was 100 KB and more of code that every wave ran once,
+// fetched from the L2 (bf16 without activation, 8192 x 1024 -> 4096: 86 -> 77 us, 57600 x 256 -> 256: 25 -> 20).  16-byte slots are XOR-swizzled by row.
+template <class T, int FN, int FM, int JC>
+__device__ __forceinline__ void store_tile(const GemmArgs& a, const f32x4 (&acc)[FN][FM], long m0, int n0, int lane, char* lds) {
+    constexpr int V = VE<T>, WN = FN * 16, CPR = WN / 4, LPR = WN / V, RPI = 64 / LPR;      // slots of a row, lanes of a row, rows of a loop step
+    const int r = lane & 15, q = lane >> 4, cl = lane % LPR, rl = lane / LPR;
+    const int col = n0 + cl * V, left = a.N - col;
+    float bias[V];
 #pragma unroll
-    for (int p = 0; p < NV; p += NR) {
-        const int col = n0 + (p + hi) * 4 * V + q * V, left = a.N - col;
-        float bias[V];
+    for (int i = 0; i < V; ++i) bias[i] = 0.0f;
+    if (a.fwd && a.bias && left > 0) load_part<float, V>(a.bias + col, left, bias);
 #pragma unroll
-        for (int i = 0; i < V; ++i) bias[i] = 0.0f;
-        if (a.fwd && a.bias && left > 0) load_part<float, V>(a.bias + col, left, bias);
+    for (int j0 = 0; j0 < FM; j0 += JC) {
 #pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            float v[NR][V];
+        for (int j = 0; j < JC; ++j)
 #pragma unroll
-            for (int u = 0; u < NR; ++u)
+            for (int f = 0; f < FN; ++f) {
+                const int slot = sizeof(T) == 2 ? 8 * (f >> 1) + 2 * q + (f & 1) : 4 * f + q, row = j * 16 + r;
+                *reinterpret_cast<f32x4*>(lds + (row * CPR + (slot ^ (row & (CPR - 1)))) * 16) = acc[f][j0 + j];
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the wave's own piece: LDS serves one wave in order
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int it = 0; it < JC * 16 / RPI; ++it) {
+            const int lr = it * RPI + rl;
+            const long row = m0 + j0 * 16 + lr;
+            float v[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[u][i] = acc[V == 8 ? 2 * (p + u) + i / 4 : p + u][j][i & 3];
-            if constexpr (NR == 2) trade(v[0], v[1], hi);
-            if (left <= 0) continue;
+            for (int u = 0; u < V / 4; ++u) {
+                const f32x4 t = *reinterpret_cast<const f32x4*>(lds + (lr * CPR + ((cl * (V / 4) + u) ^ (lr & (CPR - 1)))) * 16);
 #pragma unroll
-            for (int u = 0; u < NR; ++u) {
-                const long row = m0 + j * 16 + r0 + 8 * u;
-                if (row >= a.M) continue;
-                if (a.partial) {
-                    store_part<float, V>((float*)a.C + ((long)blockIdx.y * a.M + row) * a.N + col, left, v[u]);
-                } else if (!a.fwd) {
+                for (int i = 0; i < 4; ++i) v[4 * u + i] = t[i];
+            }
+            if (row >= a.M || left <= 0) continue;
+            if (a.partial) {
+                store_part<float, V>((float*)a.C + ((long)blockIdx.y * a.M + row) * a.N + col, left, v);
+            } else if (!a.fwd) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) v[u][i] *= a.alpha;
-                    store_part<T, V>((T*)a.C + row * a.ldc + col, left, v[u]);
-                } else {
-                    float res[V];
+                for (int i = 0; i < V; ++i) v[i] *= a.alpha;
+                store_part<T, V>((T*)a.C + row * a.ldc + col, left, v);
+            } else {
+                float res[V];
 #pragma unroll
-                    for (int i = 0; i < V; ++i) res[i] = 0.0f;
-                    if (a.res) load_part<T, V>((const T*)a.res + row * a.ldr + col, left, res);
-                    finish<T, V>(a, row, col, left, v[u], bias, res);
-                }
+                for (int i = 0; i < V; ++i) res[i] = 0.0f;
+                if (a.res) load_part<T, V>((const T*)a.res + row * a.ldr + col, left, res);
+                finish<T, V>(a, row, col, left, v, bias, res);
             }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
 // ---- the tile kernel --------------------------------------------------------------------------------------------------------------------
+// Any size, alignment and type: 128 (64) rows by 128 (64, 32) columns, 4 waves, two stages of 128-byte steps; tiles pass through registers, where edge pieces
+// are trimmed.  Bound by the matrix cores for large sizes (8192 x 1024 -> 4096: fp32 603 us = 114 TFLOP/s, bf16 133 us), by latency for small ones
+// (5003 x 177 -> 93 fp16: y 10.0, dx 6.4, dw 8.4 + 4.2 us to join 39 splits).
 template <class T, bool AKC, bool BKC, int BM, int BN, int WGM>
 __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
-    constexpr int WGN = 4 / WGM, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16, KS = sizeof(T) == 2 ? 2 : 2;
+    constexpr int WGN = 4 / WGM, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
     constexpr int ABYTES = BM * 128, BBYTES = BN * 128;
     __shared__ __attribute__((aligned(16))) char lds[2 * (ABYTES + BBYTES)];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WGN, wn = wave % WGN;
@@ -333,7 +347,7 @@ __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
         const char* la = lds + cur * ABYTES;
         const char* lb = lds + 2 * ABYTES + cur * BBYTES;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
+        for (int ks = 0; ks < 2; ++ks) {
             typename Mma<T>::Frag fa[FM], fb[FN];
 #pragma unroll
             for (int j = 0; j < FM; ++j) fa[j] = frag<T, AKC, BM, false>(la, wm * WM, j, ks, lane);
@@ -347,7 +361,8 @@ __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
         }
         __syncthreads();
     }
-    store_tile<T>(a, acc, m0 + wm * WM, n0 + wn * WN, lane);
+    static_assert(4 * WM * WN * 4 <= 2 * (ABYTES + BBYTES), "the waves' tiles fit the stages");
+    store_tile<T, FN, FM, FM>(a, acc, m0 + wm * WM, n0 + wn * WN, lane, lds + wave * (WM * WN * 4));
 }
 
 // ---- the wide tile kernel: 256 x 256 (16-bit) or 256 x 128 ------------------------------------------------------------------------------------
@@ -430,7 +445,7 @@ __global__ __launch_bounds__(512) void k_gemm_wide(GemmArgs a) {
         __builtin_amdgcn_s_waitcnt(0x0f70);
         __syncthreads();
     }
-    store_tile<T>(a, acc, m0 + wm * WM, n0 + wn * 64, lane);
+    store_tile<T, 4, FM, FM / 2>(a, acc, m0 + wm * WM, n0 + wn * 64, lane, wide_lds + wave * (WM / 2 * 256));
 }
 
 // ---- joining the splits of the contracted index: C = epilogue(sum of the partials), 4 columns a thread, L lanes over the splits -------------------
@@ -482,6 +497,7 @@ __global__ __launch_bounds__(NT) void k_join(GemmArgs a, const float* __restrict
 // y of MR rows is bound by reading w (and, for one row, by the launch).  A lane owns 16 bytes of columns and every KL-th row of w, so a workgroup
 // covers `lanes` x 16 bytes of columns and the whole contracted index: no partials in memory, one launch.  Narrow column runs give enough
 // workgroups; those that share a cache line of w run on one XCD and meet in its L2.  The KL partial sums of a column are a tree in LDS.
+// 1 x 1024 -> 4096 bf16: 5.0 us (8.4 MB: 1.7 us at the memory's rate; the rest is the launch and one round of latency).
 template <class T, int MR>
 __global__ __launch_bounds__(NT) void k_few(GemmArgs a, int lanes) {
     constexpr int V = VE<T>;
@@ -546,6 +562,7 @@ __global__ __launch_bounds__(NT) void k_few(GemmArgs a, int lanes) {
 // x w for cin <= 16-byte steps KS of the contracted index, cout <= 16 FN: bound by the rows' bytes.  A wave takes 16 rows at a time and needs no
 // other wave: x goes from memory straight into fragments (a lane's 16 bytes ARE the fragment), the next rows' while this row's products run, and
 // only the weights sit in LDS, loaded once per workgroup.  16-row steps read KS * FN KB of LDS per KS KB of x: 1/6 of the LDS rate at the memory's.
+// Measured, 898704 rows: 64 -> 64 bf16 with swish and residual 62 - 66 us = 5.2 - 5.6 TB/s, 64 -> 1 fp32 37 us (x partly cached; 44 cold = 5.3 TB/s).
 template <class T> constexpr int KSTEP = 4 * VE<T>;           // contracted elements of one fragment step: 32 or 16
 
 // 16 rows of an array: the wave's row 0 is a scalar base, a lane's place in them a 32-bit byte offset that never changes (the narrow kernels take pitches
@@ -650,7 +667,8 @@ __global__ __launch_bounds__(NT) void k_narrow(GemmArgs a) {
         if (FULL && a.res) load_res(nres, base + step * 16);
         x.trim(K, q);
         int here = 0;
-        asm volatile("" : "+v"(here));        // the weights are read from LDS for every 16 rows: kept in registers they cost a wave per SIMD (fp32 64 -> 64: 144 -> 135 us)
+        // the weights are read from LDS for every 16 rows: kept in registers they cost a wave per SIMD (fp32 64 -> 64: 144 -> 135 us)
+        asm volatile("" : "+v"(here));
         f32x4 acc[FN][1];
 #pragma unroll
         for (int f = 0; f < FN; ++f) acc[f][0] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -715,7 +733,9 @@ __global__ __launch_bounds__(NT) void k_narrow(GemmArgs a) {
 //   z = x w + b again from the x it reads anyway (cheaper than 4 bytes per output to write and read),  dz = dy act'(z),
 //   dx = dz w^T: a lane's results of the first product are 8 (4) consecutive columns of one row = exactly the operand fragment of this one,
 //   dw += x^T dz: both tiles go through a wave-private piece of LDS and come back transposed; the sums stay in registers for the whole kernel.
-// x and dy are read once, dx written once; per workgroup one record [cin][cout] + column sums of dz leaves for k_join.
+// x and dy are read once, dx written once; per workgroup one record [cin][cout] + column sums of dz leaves for k_join.  Bound by memory and, with an
+// activation, by how few waves its registers leave (2 per SIMD): 898704 x 64 -> 64 bf16 swish 73 - 77 us = 4.5 - 4.7 TB/s, fp32 229 us (bound by the fp32
+// matrix rate: 3 products of 7.4 GFLOP).
 struct NarrowBwd {
     const void* x; const void* dy; const void* w; const float* bias; const float* z; void* dx; float* part;
     long M, ldx, ldy, ldw; int K, N, act; float scale;
@@ -940,6 +960,7 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
 }
 
 // ---- wide backward: dz = dy act'(z), and the column sums of dz -----------------------------------------------------------------------------------
+// Bound by memory: 57600 x 128 fp32 17 - 21 us = 4.2 - 5.3 TB/s (the plain products then read dz twice; forming it inside them would read dy and z as often).
 struct DzArgs {
     const void* dy; const float* z; void* dz; float* part;
     long rows, dpitch; int N, act;
@@ -993,17 +1014,14 @@ int bn_of(long N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }       // column 
 // row tile: 64 rows where 128 would leave CUs without a tile (5003 x 93 -> 177: 8.7 -> 6.2 us; but 8192 x 1024 -> 4096: 133 -> 159, twice the reads of w)
 int bm_of(long M, long N) { return bn_of(N) == 128 && ((M + 127) / 128) * ((N + 127) / 128) < 256 ? 64 : 128; }
 // the wide kernel's columns (0: not for this product): 256 for 16-bit types where its tiles fill the CUs, or do with the contracted index split into
-// runs of at least 1024; 128 where those fill most of them
+// runs of at least 1024; 128 where those fill most of them (4096 x 1024 -> 1024, 128 tiles: bf16 25 -> 20 us, but fp32, bound by the matrix cores, 94 -> 129)
 constexpr long WIDE_PITCH = 1L << 21;                         // 256 rows of them fit a 32-bit byte offset
-#ifndef W128
-#define W128 192
-#endif
 long wide_tiles(long M, long N, long bn) { return ((M + 255) / 256) * ((N + bn - 1) / bn); }
 int wide_cols(long M, long N, long K, int bytes) {
     if (K % (128 / bytes) || M < 256 || N < 128) return 0;
     const long runs = std::max<long>(1, K / 1024);
     if (bytes == 2 && N >= 256 && wide_tiles(M, N, 256) * runs >= 192) return 256;
-    return wide_tiles(M, N, 128) >= W128 ? 128 : 0;
+    return wide_tiles(M, N, 128) >= (bytes == 2 ? 96 : 192) ? 128 : 0;
 }
 // how many ways the contracted index is split: one where the tiles fill the CUs; else so that one workgroup per CU runs, two where the index is long
 // (4096 x 1024 -> 1024 bf16: y 23 us with one, 34 with two; dw of 65536 x 512 -> 256: 76 us with one, 56 with two), each with at least `least` of it,
@@ -1272,7 +1290,7 @@ ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void*
     BwdWs w{};
     if (d->rows > 0) {
         w = linear_ws(d, !again);
-        if (!d_dy || ((d_dw || again) && !d_x) || ((d_dx || again) && !d_w) || !d_ws) return c->fail(TTC_ERR_ARG, "linear_backward: null pointer");
+        if (!d_dy || !d_x || !d_w || !d_ws) return c->fail(TTC_ERR_ARG, "linear_backward: null pointer");
         if ((uintptr_t)d_ws % 16) return c->fail(TTC_ERR_ARG, "linear_backward: the workspace must be 16-byte aligned");
         if (ws_bytes < w.total) return c->fail(TTC_ERR_ARG, "linear_backward: workspace smaller than ttc_linear_workspace asks for");
     }

@@ -126,6 +126,7 @@ def check_norm(ctx, x, gamma, beta, G, act, eps=1e-5, dy=None):
 NORM_SHAPES = [  # n, rows, channels, groups
     (1, 1, 1, 1), (2, 1, 64, 8), (3, 2, 6, 3), (1, 7, 23, 1), (2, 196, 64, 8), (5, 129, 40, 5), (2, 1000, 12, 4), (1, 5000, 64, 8), (70, 9, 16, 16),
     (2, 33, 512, 32), (1, 11, 4096, 8), (2, 3, 1000, 125), (1, 40, 2056, 8), (3, 257, 130, 2), (1, 30000, 8, 8), (2, 700, 257, 257),
+    (300, 512, 64, 8),
 ]
 
 
@@ -379,13 +380,19 @@ def test_refusals_on_the_device(ctx):
     assert lib.ttc_group_norm(ctx._h, C.byref(d), p, None, None, p, None, p, 8, None) == 1 and b"workspace" in lib.ttc_last_error(ctx._h)
     assert lib.ttc_group_norm(ctx._h, C.byref(d), None, None, None, p, None, p, 1 << 20, None) == 1
     assert lib.ttc_group_norm_backward(ctx._h, C.byref(d), p, 96, 16, p, None, None, p, p, None, None, p, 8, None) == 1 and b"workspace" in lib.ttc_last_error(ctx._h)
+    assert lib.ttc_group_norm(ctx._h, C.byref(d), p, None, None, p, None, p + 4, 1 << 30, None) == 1 and b"aligned" in lib.ttc_last_error(ctx._h)
     d = _lib.TTCGroupNormDesc(0, 0, 1, 6, 16, 4, 96, 16, 1e-5)
     assert lib.ttc_group_norm(ctx._h, C.byref(d), None, None, None, p, None, p, 1 << 20, None) == 1
     assert lib.ttc_group_norm_backward(ctx._h, C.byref(d), p, 96, 16, p, None, None, None, p, None, None, p, 1 << 20, None) == 1
     l = _lib.TTCLinearDesc(0, 2, 6, 16, 8, 16, 8, 8, 8, 1.0)
     assert lib.ttc_linear(ctx._h, C.byref(l), None, p, None, None, p, None, None, 0, None) == 1
     assert lib.ttc_linear_backward(ctx._h, C.byref(l), p, p, None, None, None, p, p, None, p, 1 << 20, None) == 1
+    for px, pw, dx, dw in ((None, p, p, None), (p, None, None, p)):          # one gradient alone: the narrow pass still reads all three arrays
+        l.activation = 0
+        assert lib.ttc_linear_backward(ctx._h, C.byref(l), p, px, pw, None, None, dx, dw, None, p, 1 << 20, None) == 1 and b"null" in lib.ttc_last_error(ctx._h)
+        l.activation = 2
     assert lib.ttc_linear_backward(ctx._h, C.byref(l), p, p, p, None, None, p, p, p, p, 1, None) == 1 and b"workspace" in lib.ttc_last_error(ctx._h)
+    assert lib.ttc_linear_backward(ctx._h, C.byref(l), p, p, p, None, None, p, p, p, p + 8, 1 << 30, None) == 1 and b"aligned" in lib.ttc_last_error(ctx._h)
     torch.cuda.synchronize()
 
 
