@@ -402,8 +402,8 @@ __global__ __launch_bounds__(NT) void k_gn_bwd_apply(NormArgs a) {
 
 // ---- one launch: a workgroup holds whole groups of a sample ------------------------------------------------------------------------------
 // blockIdx.x = slab of a.cols * V channels (whole groups, V divides channels / groups), blockIdx.y = sample; RU vectors a thread stay in registers
-// as stored.  14 x 14 x 64 fp32: 4.7 us against 4.2 + 4.7 by two launches; 32 x 28 x 28 x 64 fp32 6.5 against 5.5 + 6.4, backward 11 + 4 against 23;
-// 5 x 61 x 47 x 40 fp16 10.5 against 14 (with 8 vectors a thread: 14.6, too few workgroups share the chip).
+// as stored (with 8 vectors a thread 5 x 61 x 47 x 40 fp16 takes 14.6 us instead of 10.5: too few workgroups share the chip).  Bound by latency.
+// 14 x 14 x 64 fp32: 4.4 us against 7.8 by two launches; norm_resident has both sides of more sizes.
 template <class T, int V>
 struct Held {
     static constexpr int W = V * sizeof(T) >= 4 ? V * sizeof(T) / 4 : 1;
@@ -489,8 +489,7 @@ __global__ __launch_bounds__(RT) void k_gn_resident(NormArgs a) {
 }
 
 // the same for the backward pass: x is held, dy read again for dx (holding both spills: its second read comes from the L2); the sums of a channel over
-// the rows are a 32-bit tree in LDS.  direct: one sample, so its sums ARE the parameters'
-// gradients
+// the rows are a 32-bit tree in LDS.  direct: one sample, so its sums ARE the parameters' gradients
 template <class T, int V>
 __global__ __launch_bounds__(RT) void k_gn_resident_bwd(NormArgs a, int direct) {
     extern __shared__ float sf[];                  // [rpb][cols * V][2], row 0 becomes the channels' sums, row 1 the groups'
@@ -596,9 +595,15 @@ void norm_geometry(NormArgs& a, int V) {
 }
 
 // resident kernels: V divides channels / groups; the slab is all channels, halved (in whole groups) while it does not fit or while the launch has
-// fewer than 256 workgroups and the halves still read whole 64-byte pieces.  false: a single group does not fit.
+// fewer than 256 workgroups and the halves still read whole 64-byte pieces.  false: a single group does not fit, or the streaming kernels are faster:
+//  - forward: a slab's pieces of a row below 64 bytes, of more than 4 MB in all (lines fetched by several XCDs).  us resident / streaming: fp16 5 x 2867 x 40
+//    in groups of 8 8.3 / 10.2, 16 x 2867 x 64 15.4 / 11.3; fp32 8 x 1200 x 64 6.3 / 8.9, 8 x 2048 x 64 8.0 / 8.3, 32 x 2048 x 64 18.5 / 13.0, 32 x 784 x 64
+//    (64 bytes) 6.0 / 9.9.
+//  - backward: more than 13 elements a thread or a second round of workgroups (its phases wait for each other; streaming spreads them over the chip):
+//    fp16 1 x 196 x 64 9.3 / 12.9, 1 x 784 x 64 13.4 / 12.6, 5 x 2867 x 40 16.8 / 13.8, 36 x 1600 x 256 74.5 / 35.7; fp32 1 x 400 x 64 6.8 / 10.5,
+//    8 x 784 x 256 11.9 / 14.4, 32 x 2048 x 64 37.7 / 19.7, 1024 x 49 x 64 42.5 / 30.9.
 struct Slab { int v, threads, slabs; };
-bool norm_resident(NormArgs& a, int bytes, Slab* s) {
+bool norm_resident(NormArgs& a, int bytes, bool backward, Slab* s) {
     s->v = norm_vec(a.cpg, bytes);
     int groups = a.G;
     auto vecs = [&](int g) { return a.rows * (long)g * a.cpg / s->v; };
@@ -613,7 +618,9 @@ bool norm_resident(NormArgs& a, int bytes, Slab* s) {
     a.rpb = (int)std::min<long>(a.rpb, a.rows);
     s->threads = (a.cols * a.rpb + 63) / 64 * 64;
     s->slabs = (a.G + groups - 1) / groups;
-    return true;
+    const long piece = (long)groups * a.cpg;
+    if (backward) return a.rows * piece <= 13 * RT && (long)a.n * s->slabs <= 256;
+    return s->slabs == 1 || piece * bytes >= 64 || a.n * a.rows * a.C * bytes <= 4 << 20;
 }
 
 struct NormWs { size_t csum, coef, total; };
@@ -656,7 +663,7 @@ NormPlan norm_plan(const ttc_group_norm_desc* d, bool backward) {
     a.rows = d->rows; a.n = (int)d->n; a.C = d->channels; a.G = d->groups; a.cpg = d->channels / d->groups;
     a.act = d->activation; a.eps = d->eps;
     a.sn = d->x_stride; a.pitch = d->x_pitch;
-    p.resident = d->rows > 0 && norm_resident(a, bytes, &p.slab);
+    p.resident = d->rows > 0 && norm_resident(a, bytes, backward, &p.slab);
     if (!p.resident) {
         p.V = norm_vec(a.C, bytes);
         norm_geometry(a, p.V);
