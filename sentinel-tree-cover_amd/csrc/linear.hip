@@ -453,7 +453,7 @@ __global__ __launch_bounds__(512) void k_gemm_wide(GemmArgs a) {
 template <class T, int L>
 __global__ __launch_bounds__(NT) void k_join(GemmArgs a, const float* __restrict__ part, long rec, int splits, int tail, float* __restrict__ tail_out) {
     constexpr int E = NT / L;
-    __shared__ float red[L > 1 ? L : 1][E * 4];
+    __shared__ float red[4][E * 4];                    // one partial of each wave
     const int e = threadIdx.x % E, l = threadIdx.x / E;
     const int nv = (a.N + 3) / 4;
     const long vecs = a.M * nv, id = (long)blockIdx.x * E + e;
@@ -475,12 +475,19 @@ __global__ __launch_bounds__(NT) void k_join(GemmArgs a, const float* __restrict
 #pragma unroll
             for (int i = 0; i < 4; ++i) if (i < left) s[i] += part[k * rec + off + i];
     }
-    if constexpr (L > 1) {
+    if constexpr (L > 1) {                             // a wave holds 64 / E of the L lanes of an output: a tree, then the four waves in order
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[l][e * 4 + i] = s[i];
+        for (int m = E; m < 64; m <<= 1)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] += __shfl_xor(s[i], m);
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) < E)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) red[wave][e * 4 + i] = s[i];
         __syncthreads();
         if (l) return;
-        for (int k = 1; k < L; ++k)
+#pragma unroll
+        for (int k = 1; k < 4; ++k)
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[i] += red[k][e * 4 + i];
     }
