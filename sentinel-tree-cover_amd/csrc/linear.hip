@@ -462,18 +462,25 @@ __global__ __launch_bounds__(NT) void k_join(GemmArgs a, const float* __restrict
     if (id < vecs) { row = id / nv; col = (int)(id % nv) * 4; off = row * a.N + col; left = min(4, a.N - col); }
     else { col = (int)min((id - vecs) * 4, (long)tail); off = a.M * a.N + col; left = min(4, tail - col); }
     float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (left == 4) {
-#pragma unroll 4
-        for (int k = l; k < splits; k += L) {
-            float v[4];
-            load_vec<float, 4>(part + k * rec + off, v);
+    constexpr int U = L == 64 ? 8 : 4;                 // loads in flight: past the last split they read it again and are dropped
+    auto sum = [&](auto load) {
+        for (int k = l; k < splits; k += U * L) {
+            float v[U][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] += v[i];
+            for (int u = 0; u < U; ++u) load(part + min(k + u * L, splits - 1) * rec + off, v[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] += k + u * L < splits ? v[u][i] : 0.0f;
         }
+    };
+    if (left == 4) {
+        sum([](const float* p, float (&v)[4]) { load_vec<float, 4>(p, v); });
     } else if (left > 0) {
-        for (int k = l; k < splits; k += L)
+        sum([&](const float* p, float (&v)[4]) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) if (i < left) s[i] += part[k * rec + off + i];
+            for (int i = 0; i < 4; ++i) v[i] = p[min(i, left - 1)];
+        });
     }
     if constexpr (L > 1) {                             // a wave holds 64 / E of the L lanes of an output: a tree, then the four waves in order
 #pragma unroll
