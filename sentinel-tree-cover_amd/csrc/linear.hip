@@ -1038,15 +1038,19 @@ int wide_cols(long M, long N, long K, int bytes) {
     return wide_tiles(M, N, 128) >= (bytes == 2 ? 96 : 192) ? 128 : 0;
 }
 // how many ways the contracted index is split: one where the tiles fill the CUs; else so that one workgroup per CU runs, two where the index is long
-// (4096 x 1024 -> 1024 bf16: y 23 us with one, 34 with two; dw of 65536 x 512 -> 256: 76 us with one, 56 with two), each with at least `least` of it,
-// and the partials stay under 64 MB
-int gemm_splits(long M, long N, long K, long least, int bytes) {
-    const long fit = std::max<long>(1, (64L << 20) / (M * N * 4));
+// (4096 x 1024 -> 1024 bf16: y 23 us with one, 34 with two; dw of 65536 x 512 -> 256: 76 us with one, 56 with two), and the partials stay under 64 MB.
+// A split and its join cost about 5 us.  16-bit products below 384 take none (dx of 1000 x 1024 -> 256: 7.0 us against 12.7) and up to 4096 as many as
+// keep the partials under 4 MB (64 x 1024 -> 4096: 12.0 us by four, 13.9 by eight), two of a thousand in any case (dw of 1500 x 1000 -> 1000: 23 us against
+// 31); fp32, with a quarter of their matrix rate, splits down to 64 (64 x 512 -> 512: 9.8 us against 12.0 at 128; 16 x 1024 -> 4096 by eight 14, four 19)
+int gemm_splits(long M, long N, long K, int bytes) {
+    const long bytes_one = M * N * 4;
+    long fit = std::max<long>(1, (64L << 20) / bytes_one);
     if (const int wn = wide_cols(M, N, K, bytes)) return (int)std::max<long>(1, std::min<long>({256 / wide_tiles(M, N, wn), K / 1024, fit}));
+    if (bytes == 2 && K < 384) return 1;
+    if (bytes == 2 && K <= 4096) fit = std::min(fit, std::max<long>(K >= 1024 ? 2 : 1, (4L << 20) / bytes_one));
     const long bm = bm_of(M, N), tiles = ((M + bm - 1) / bm) * ((N + bn_of(N) - 1) / bn_of(N));
-    return (int)std::max<long>(1, std::min<long>({(K > 4096 ? 512 : 256) / tiles, K / least, fit}));
+    return (int)std::max<long>(1, std::min<long>({(K > 4096 ? 512 : 256) / tiles, K / (bytes == 2 ? 128 : 64), fit}));
 }
-constexpr long LEAST_K = 128, LEAST_ROWS = 128;
 
 template <class T>
 void join_launch(const GemmArgs& a, const float* part, long rec, int splits, int tail, float* tail_out, hipStream_t s) {
@@ -1187,9 +1191,9 @@ BwdWs linear_ws(const ttc_linear_desc* d, bool have_z) {
     w.dz = act && !have_z ? up(cells * sizeof(float)) : 0;
     w.sums = w.dz + (act ? up(cells * dtype_bytes(d->dtype)) : 0);
     w.part = w.sums + up((size_t)w.blocks * d->cout * sizeof(float));
-    const size_t zs = act && !have_z ? (size_t)gemm_splits(d->rows, d->cout, d->cin, LEAST_K, dtype_bytes(d->dtype)) : 1;
-    w.dx_splits = gemm_splits(d->rows, d->cin, d->cout, LEAST_K, dtype_bytes(d->dtype));
-    w.dw_splits = gemm_splits(d->cin, d->cout, d->rows, LEAST_ROWS, dtype_bytes(d->dtype));
+    const size_t zs = act && !have_z ? (size_t)gemm_splits(d->rows, d->cout, d->cin, dtype_bytes(d->dtype)) : 1;
+    w.dx_splits = gemm_splits(d->rows, d->cin, d->cout, dtype_bytes(d->dtype));
+    w.dw_splits = gemm_splits(d->cin, d->cout, d->rows, dtype_bytes(d->dtype));
     size_t part = 0;
     if (zs > 1) part = zs * cells;
     if (w.dx_splits > 1) part = std::max(part, (size_t)w.dx_splits * d->rows * d->cin);
@@ -1254,7 +1258,7 @@ ttc_status ttc_linear_workspace(const ttc_linear_desc* d, int32_t backward, size
     if (linear_check(d)) return TTC_ERR_ARG;
     if (d->rows == 0) return TTC_OK;
     if (backward) { *bytes = linear_ws(d, backward == TTC_LINEAR_HAVE_PREACT).total; return TTC_OK; }
-    const int sp = narrow_fwd(d) || few_rows(d) ? 1 : gemm_splits(d->rows, d->cout, d->cin, LEAST_K, dtype_bytes(d->dtype));
+    const int sp = narrow_fwd(d) || few_rows(d) ? 1 : gemm_splits(d->rows, d->cout, d->cin, dtype_bytes(d->dtype));
     if (sp > 1) *bytes = (size_t)sp * d->rows * d->cout * sizeof(float);
     return TTC_OK;
 }
@@ -1271,7 +1275,7 @@ ttc_status ttc_linear(ttc_ctx* c, const ttc_linear_desc* d, const void* d_x, con
         return c->fail(TTC_ERR_ARG, "linear: res_pitch must be at least cout");
     if (d->rows == 0) return TTC_OK;
     const bool narrow = narrow_fwd(d), few = few_rows(d);
-    const int sp = narrow || few ? 1 : gemm_splits(d->rows, d->cout, d->cin, LEAST_K, dtype_bytes(d->dtype));
+    const int sp = narrow || few ? 1 : gemm_splits(d->rows, d->cout, d->cin, dtype_bytes(d->dtype));
     if (!d_x || !d_w || !d_y || (sp > 1 && !d_ws)) return c->fail(TTC_ERR_ARG, "linear: null pointer");
     if (sp > 1 && (uintptr_t)d_ws % 16) return c->fail(TTC_ERR_ARG, "linear: the workspace must be 16-byte aligned");
     if (sp > 1 && ws_bytes < (size_t)sp * d->rows * d->cout * sizeof(float))
@@ -1338,7 +1342,7 @@ ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void*
             GemmArgs a = fwd_args(d, d_x, d_w);
             GemmArgs zf = a;
             zf.fwd = 1; zf.act = TTC_ACT_NONE; zf.alpha = 1.0f; zf.bias = d_bias; zf.C = nullptr; zf.preact = (float*)ws;
-            gemm_launch<T, true, false>(zf, gemm_splits(d->rows, d->cout, d->cin, LEAST_K, dtype_bytes(d->dtype)), (float*)(ws + w.part), s);
+            gemm_launch<T, true, false>(zf, gemm_splits(d->rows, d->cout, d->cin, dtype_bytes(d->dtype)), (float*)(ws + w.part), s);
             z = (const float*)ws;
         }
         const T* dz = act ? (const T*)(ws + w.dz) : (const T*)d_dy;     // without an activation dz is dy itself; the scale is in the epilogues either way
