@@ -446,8 +446,8 @@ ttc_status ttc_s1_to_db(ttc_ctx* ctx, const uint16_t* d_u16, int32_t T, int32_t 
  *                   (TF layout [1, 1, cin, cout]); the graph's 1x1 sigmoid head (src/train/train-model.py:226-231) is
  *                   linear(late, head/kernel, head/bias, sigmoid)
  * Arrays are fp32, fp16 or bf16 (one type per call); gamma, beta, bias, the statistics and the gradients of gamma, beta and bias are always
- * float32.  Sums and statistics are held in 32 bits or more, results are rounded once (and dz of ttc_linear_backward once to the arrays' type,
- * as operand of the two matrix products); no atomics: two runs give the same bits.
+ * float32.  Sums and statistics are held in 32 bits or more, results are rounded once (dz of
+ * ttc_linear_backward is an operand of two matrix products as a pair of 16-bit values: 16 bits for bf16, 22 for fp16); no atomics: two runs give the same bits.
  * Nothing here uses the context's workspace, weights or window geometry: the caller passes the scratch memory the *_workspace query
  * names (16-byte aligned), so calls on several streams and calls captured into several graphs do not share any.  No call allocates, synchronises or
  * copies; all of them can be captured into a graph.  Rows need unit channel stride and may be a slice of wider rows; a row may start at any

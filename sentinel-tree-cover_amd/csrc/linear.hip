@@ -31,6 +31,7 @@ constexpr int NT = 256;
 
 struct GemmArgs {
     const void* A; const void* B;
+    const void* Alo; const void* Blo;   // the low halves of a pair (dz_pair), of A or of B, in the same strides; or none
     long lda, ldb;
     long M; int N; long K;          // C is [M, N], K contracted
     long k_per;                     // contracted range of a split (blockIdx.y)
@@ -73,6 +74,30 @@ __device__ __forceinline__ void mma_block(f32x4 (&acc)[I][J], const typename Mma
         for (int i = 0; i < I; ++i)
 #pragma unroll
             for (int j = 0; j < J; ++j) acc[i][j] = Mma<T>::run(b[i], a[j], acc[i][j]);
+    }
+}
+
+// dz = dy act'(z) is a 32-bit value and an operand of two products in the arrays' type.  In 16 bits it goes in as the pair hi + lo / LO_UP, multiplied one
+// after the other: rounded once instead, dx and dw were 1.4 times as far from their 64-bit values as their own rounding takes them (bf16 2.35e-3 against 1.66e-3).
+// The pair holds 16 (bf16) or 22 bits (fp16).  fp16 has a narrow range: the value is halved, so that a slope up to 1.13 does not overflow it, and its low
+// half, 11 bits further down, comes up by 2^11, out of the subnormals (smallest piece 2^-35).
+template <class T> constexpr float DZ_DOWN = std::is_same_v<T, f16> ? 0.5f : 1.0f;      // undone by the products' alpha
+template <class T> constexpr float LO_UP = std::is_same_v<T, f16> ? 2048.0f : 1.0f;
+template <class T>
+__device__ __forceinline__ void dz_pair(float v, T* hi, T* lo) {
+    *hi = (T)v;
+    const float d = (v - (float)*hi) * LO_UP<T>;
+    *lo = (T)(fabsf(d) < INFINITY ? d : 0.0f);     // an infinite or NaN v stays in hi alone
+}
+
+// the products of the low halves are summed: down to the high ones' scale
+template <class T, int I, int J>
+__device__ __forceinline__ void lo_done(f32x4 (&acc)[I][J]) {
+    if constexpr (LO_UP<T> != 1.0f) {
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int j = 0; j < J; ++j) acc[i][j] *= 1.0f / LO_UP<T>;
     }
 }
 
@@ -311,7 +336,8 @@ __device__ __forceinline__ void store_tile(const GemmArgs& a, const f32x4 (&acc)
 // Any size, alignment and type: 128 (64) rows by 128 (64, 32) columns, 4 waves, two stages of 128-byte steps; tiles pass through registers, where edge pieces
 // are trimmed.  Bound by the matrix cores for large sizes (8192 x 1024 -> 4096: fp32 603 us = 114 TFLOP/s, bf16 133 us), by latency for small ones
 // (5003 x 177 -> 93 fp16: y 10.0, dx 6.4, dw 8.4 + 4.2 us to join 39 splits).
-template <class T, bool AKC, bool BKC, int BM, int BN, int WGM>
+// PAIR: A or B comes as a pair of 16-bit halves (dz): the range is walked twice, the low halves first
+template <class T, bool AKC, bool BKC, int BM, int BN, int WGM, bool PAIR>
 __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
     constexpr int WGN = 4 / WGM, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
     constexpr int ABYTES = BM * 128, BBYTES = BN * 128;
@@ -323,8 +349,9 @@ __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
     const long m0 = (long)(tile / a.nt) * BM;
     const int n0 = (tile % a.nt) * BN;
     const long k0 = blockIdx.y * a.k_per, k1 = min(k0 + a.k_per, a.K);
-    const T* A = (const T*)a.A;
-    const T* B = (const T*)a.B;
+    const T* A = (const T*)(PAIR && a.Alo ? a.Alo : a.A);
+    const T* B = (const T*)(PAIR && a.Blo ? a.Blo : a.B);
+    bool low = PAIR;
     Stage<T, AKC, BM> sa;
     Stage<T, BKC, BN> sb;
     f32x4 acc[FN][FM];
@@ -338,11 +365,14 @@ __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
     sb.store(lds + 2 * ABYTES, n0, a.N, k0, k1, tid);
     __syncthreads();
     int cur = 0;
-    for (long k = k0; k < k1; k += BKE<T>, cur ^= 1) {
-        const bool more = k + BKE<T> < k1;
+    for (long k = k0;; cur ^= 1) {
+        const bool turn = low && k + BKE<T> >= k1;           // a pair's last low step: the high halves follow from k0
+        const bool more = turn || k + BKE<T> < k1;
+        k = turn ? k0 : k + BKE<T>;
+        if (PAIR && turn) { A = (const T*)a.A; B = (const T*)a.B; }
         if (more) {
-            sa.load(A, a.lda, m0, a.M, k + BKE<T>, k1, tid);
-            sb.load(B, a.ldb, n0, a.N, k + BKE<T>, k1, tid);
+            sa.load(A, a.lda, m0, a.M, k, k1, tid);
+            sb.load(B, a.ldb, n0, a.N, k, k1, tid);
         }
         const char* la = lds + cur * ABYTES;
         const char* lb = lds + 2 * ABYTES + cur * BBYTES;
@@ -355,11 +385,13 @@ __global__ __launch_bounds__(NT) void k_gemm(GemmArgs a) {
             for (int i = 0; i < FN; ++i) fb[i] = frag<T, BKC, BN, true>(lb, wn * WN, i, ks, lane);
             mma_block<T>(acc, fb, fa);
         }
+        if (PAIR && turn) { lo_done<T>(acc); low = false; }
         if (more) {                                // the other half was last read before the previous barrier
-            sa.store(lds + (cur ^ 1) * ABYTES, m0, a.M, k + BKE<T>, k1, tid);
-            sb.store(lds + 2 * ABYTES + (cur ^ 1) * BBYTES, n0, a.N, k + BKE<T>, k1, tid);
+            sa.store(lds + (cur ^ 1) * ABYTES, m0, a.M, k, k1, tid);
+            sb.store(lds + 2 * ABYTES + (cur ^ 1) * BBYTES, n0, a.N, k, k1, tid);
         }
         __syncthreads();
+        if (!more) break;
     }
     static_assert(4 * WM * WN * 4 <= 2 * (ABYTES + BBYTES), "the waves' tiles fit the stages");
     store_tile<T, FN, FM, FM>(a, acc, m0 + wm * WM, n0 + wn * WN, lane, lds + wave * (WM * WN * 4));
@@ -399,7 +431,7 @@ struct WideTile {
     }
 };
 constexpr int WIDE_LDS(int bn) { return 2 * (256 + bn) * 128; }
-template <class T, bool AKC, bool BKC, int BN>
+template <class T, bool AKC, bool BKC, int BN, bool PAIR>
 __global__ __launch_bounds__(512) void k_gemm_wide(GemmArgs a) {
     extern __shared__ __attribute__((aligned(16))) char wide_lds[];      // A0 A1 B0 B1
     constexpr int TA = 256 * 128, TB = BN * 128, WGN = BN / 64, WM = 256 / (8 / WGN), FM = WM / 16;
@@ -409,8 +441,9 @@ __global__ __launch_bounds__(512) void k_gemm_wide(GemmArgs a) {
     const long m0 = (long)(tile / a.nt) * 256;
     const int n0 = (tile % a.nt) * BN;
     const long k0 = blockIdx.y * a.k_per, k1 = min(k0 + a.k_per, a.K);
-    const T* A = (const T*)a.A;
-    const T* B = (const T*)a.B;
+    const T* A = (const T*)(PAIR && a.Alo ? a.Alo : a.A);
+    const T* B = (const T*)(PAIR && a.Blo ? a.Blo : a.B);
+    bool low = PAIR;
     f32x4 acc[4][FM];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -426,10 +459,13 @@ __global__ __launch_bounds__(512) void k_gemm_wide(GemmArgs a) {
     __builtin_amdgcn_s_waitcnt(0x0f70);            // vmcnt(0): this wave's pieces have landed; the barrier makes that everyone's
     __syncthreads();
     int cur = 0;
-    for (long k = k0; k < k1; k += BKE<T>, cur ^= 1) {
-        if (k + BKE<T> < k1) {                     // the other stage was last read before the barrier
-            ta.fetch(A, a.lda, m0, k + BKE<T>, lds0 + (cur ^ 1) * TA, wave);
-            tb.fetch(B, a.ldb, n0, k + BKE<T>, lds0 + 2 * TA + (cur ^ 1) * TB, wave);
+    for (long k = k0;; cur ^= 1) {
+        const bool turn = low && k + BKE<T> >= k1, more = turn || k + BKE<T> < k1;           // as in k_gemm
+        k = turn ? k0 : k + BKE<T>;
+        if (PAIR && turn) { A = (const T*)a.A; B = (const T*)a.B; }
+        if (more) {                                // the other stage was last read before the barrier
+            ta.fetch(A, a.lda, m0, k, lds0 + (cur ^ 1) * TA, wave);
+            tb.fetch(B, a.ldb, n0, k, lds0 + 2 * TA + (cur ^ 1) * TB, wave);
         }
         const char* la = wide_lds + cur * TA;
         const char* lb = wide_lds + 2 * TA + cur * TB;
@@ -442,8 +478,10 @@ __global__ __launch_bounds__(512) void k_gemm_wide(GemmArgs a) {
             for (int j = 0; j < FM; ++j) fa[j] = frag<T, AKC, 256, false>(la, wm * WM, j, ks, lane);
             mma_block<T>(acc, fb, fa);
         }
+        if (PAIR && turn) { lo_done<T>(acc); low = false; }
         __builtin_amdgcn_s_waitcnt(0x0f70);
         __syncthreads();
+        if (!more) break;
     }
     store_tile<T, 4, FM, FM / 2>(a, acc, m0 + wm * WM, n0 + wn * 64, lane, wide_lds + wave * (WM / 2 * 256));
 }
@@ -747,30 +785,38 @@ __global__ __launch_bounds__(NT) void k_narrow(GemmArgs a) {
 //   z = x w + b again from the x it reads anyway (cheaper than 4 bytes per output to write and read),  dz = dy act'(z),
 //   dx = dz w^T: a lane's results of the first product are 8 (4) consecutive columns of one row = exactly the operand fragment of this one,
 //   dw += x^T dz: both tiles go through a wave-private piece of LDS and come back transposed; the sums stay in registers for the whole kernel.
+// In 16 bits with an activation dz is a pair (dz_pair): the last two products run on its low half too, with the same fragments of w and x.
 // x and dy are read once, dx written once; per workgroup one record [cin][cout] + column sums of dz leaves for k_join.  Bound by memory and, with an
-// activation, by how few waves its registers leave (2 per SIMD): 898704 x 64 -> 64 bf16 swish 73 - 77 us = 4.5 - 4.7 TB/s, fp32 229 us (bound by the fp32
-// matrix rate: 3 products of 7.4 GFLOP).
+// activation, by how few waves its registers leave (2 per SIMD): 898704 x 64 -> 64 bf16 without an activation 73 us = 4.7 TB/s, with swish 94 - 102 (80 - 84 on a
+// single rounded dz); fp32 219 - 229 us, 2/3 of the fp32 matrix rate (3 products of 7.4 GFLOP).
 struct NarrowBwd {
     const void* x; const void* dy; const void* w; const float* bias; const float* z; void* dx; float* part;
     long M, ldx, ldy, ldw; int K, N, act; float scale;
     int want_dw, want_db;
 };
+// image of w | per wave a tile of x, one of dz, of a pair one of the low halves | bias; at the end the sums of all four waves
+template <class T, int KS, int NS, bool PAIR>
+constexpr int NARROW_BWD_LDS() {
+    const int kp = KS * KSTEP<T>, np = NS * KSTEP<T>, rows = sizeof(T) == 2 ? 32 : 16;
+    const int run = (kp * np + 4 * rows * (kp + (PAIR ? 2 : 1) * np)) * (int)sizeof(T) + np * 4, red = (kp * np + np) * 4;
+    return run > red ? run : red;
+}
 // FULL: cin and cout are exactly the padded sides and the preact is formed again (as in k_narrow: no masks, no second set of addresses).
-template <class T, int KS, int NS, bool FULL>
+// PAIR: 16-bit with an activation; without one dz is dy itself, and the registers of z and of the pair are free.
+template <class T, int KS, int NS, bool FULL, bool PAIR>
 __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) void k_narrow_bwd(NarrowBwd a) {
     constexpr int KP = KS * KSTEP<T>, NP = NS * KSTEP<T>, FK = KP / 16, FN = NP / 16;
     constexpr bool H16 = sizeof(T) == 2;
+    static_assert(H16 || !PAIR);
     constexpr int RF = H16 ? 2 : 1, RW = 16 * RF, V = VE<T>;
     typedef typename Mma<T>::Frag Frag;
     constexpr int TX = RW * KP * sizeof(T), TZ = RW * NP * sizeof(T), IMG = KP * NP * sizeof(T);
-    constexpr int REDB = KP * NP * 4 + NP * 4;
-    constexpr int LDSB = IMG + 4 * (TX + TZ) > REDB ? IMG + 4 * (TX + TZ) : REDB;
-    __shared__ __attribute__((aligned(16))) char lds[LDSB];
+    extern __shared__ __attribute__((aligned(16))) char lds[];       // NARROW_BWD_LDS
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, q = lane >> 4;
     const Rows16 ax = rows16<T>(a.x, a.ldx, a.M), ad = rows16<T>(a.dy, a.ldy, a.M);
     char* lw = lds;
-    char* lx = lds + IMG + wave * (TX + TZ);
-    char* lz = lx + TX;
+    char* lx = lds + IMG + wave * (TX + (PAIR ? 2 : 1) * TZ);
+    char* lz = lx + TX;                                      // the pair's high tile, then its low one
     const long groups = (a.M + RW - 1) / RW, step = (long)gridDim.x * 4;
     long g = (long)blockIdx.x * 4 + wave;
     RowFrag<T, KS, FULL> x0[RF], x1[RF];
@@ -781,15 +827,13 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
         d0[h].load(ad, g * RW + h * 16, r, a.N, q);
     }
     load_image<T, NP>(lw, (const T*)a.w, a.ldw, a.K, a.N, KP, tid, NT);
-    float bias[NS][V], db[NS][V];
+    float* lb = reinterpret_cast<float*>(lds + IMG + 4 * (TX + (PAIR ? 2 : 1) * TZ));        // bias: beside the sums its registers spill
+    for (int i = tid; i < NP; i += NT) lb[i] = a.bias && i < a.N ? a.bias[i] : 0.0f;
+    float db[NS][V];
 #pragma unroll
     for (int p = 0; p < NS; ++p)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int col = p * KSTEP<T> + q * V + i;
-            bias[p][i] = a.bias && col < a.N ? a.bias[col] : 0.0f;
-            db[p][i] = 0.0f;
-        }
+        for (int i = 0; i < V; ++i) db[p][i] = 0.0f;
     f32x4 dw[FN][FK];
 #pragma unroll
     for (int i = 0; i < FN; ++i)
@@ -815,8 +859,8 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
 #pragma unroll
                 for (int s = 0; s < KS; ++s) x[h].v[s] = make_uint4(0, 0, 0, 0);
             }
-            Frag dz[NS];
-            if (a.act == TTC_ACT_NONE) {
+            Frag dz[NS], dl[NS];                             // dl: the pair's low halves
+            if ((H16 && !PAIR) || (!H16 && a.act == TTC_ACT_NONE)) {
 #pragma unroll
                 for (int p = 0; p < NS; ++p) {
                     dz[p] = __builtin_bit_cast(Frag, d[h].v[p]);
@@ -837,9 +881,7 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
                     }
                 } else {
 #pragma unroll
-                    for (int f = 0; f < FN; ++f)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) z[f][0][i] = bias[H16 ? f >> 1 : f][H16 ? 4 * (f & 1) + i : i];
+                    for (int f = 0; f < FN; ++f) z[f][0] = *reinterpret_cast<const f32x4*>(lb + (H16 ? 32 * (f >> 1) + 8 * q + 4 * (f & 1) : 16 * f + 4 * q));
 #pragma unroll
                     for (int s = 0; s < KS; ++s) {
                         Frag fw[FN];
@@ -858,8 +900,15 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
                     slope_vec<V>(t, zz, a.act);
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
+                        t[i] *= DZ_DOWN<T>;
                         db[p][i] += t[i];
-                        dz[p][i] = (T)t[i];                  // operands of the two products have the arrays' type: the one rounding of dz
+                        if constexpr (PAIR) {
+                            T hi, lo;
+                            dz_pair<T>(t[i], &hi, &lo);
+                            dz[p][i] = hi; dl[p][i] = lo;
+                        } else {
+                            dz[p][i] = (T)t[i];
+                        }
                     }
                 }
             }
@@ -867,15 +916,19 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
                 f32x4 o[FK][1];
 #pragma unroll
                 for (int f = 0; f < FK; ++f) o[f][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+                auto times_w = [&](const Frag (&z)[NS]) {
 #pragma unroll
-                for (int p = 0; p < NS; ++p) {
-                    Frag fw[FK];
-                    const Frag fr[1] = {dz[p]};
+                    for (int p = 0; p < NS; ++p) {
+                        Frag fw[FK];
+                        const Frag fr[1] = {z[p]};
 #pragma unroll
-                    for (int f = 0; f < FK; ++f)
-                        fw[f] = __builtin_bit_cast(Frag, *reinterpret_cast<const uint4*>(lw + fc_byte<T, NP>(free_of<T, true>(f, r), p * KSTEP<T> + q * V)));
-                    mma_block<T>(o, fw, fr);
-                }
+                        for (int f = 0; f < FK; ++f)
+                            fw[f] = __builtin_bit_cast(Frag, *reinterpret_cast<const uint4*>(lw + fc_byte<T, NP>(free_of<T, true>(f, r), p * KSTEP<T> + q * V)));
+                        mma_block<T>(o, fw, fr);
+                    }
+                };
+                if constexpr (PAIR) { times_w(dl); lo_done<T>(o); }
+                times_w(dz);
                 const int hi = KS == 1 ? 0 : r >> 3;
 #pragma unroll
                 for (int p = 0; p < KS; p += 2) {
@@ -912,6 +965,9 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
                 for (int s = 0; s < KS; ++s) *reinterpret_cast<uint4*>(lx + fc_byte<T, KP>(h * 16 + r, s * KSTEP<T> + q * V)) = x[h].v[s];
 #pragma unroll
                 for (int p = 0; p < NS; ++p) *reinterpret_cast<uint4*>(lz + fc_byte<T, NP>(h * 16 + r, p * KSTEP<T> + q * V)) = __builtin_bit_cast(uint4, dz[p]);
+                if constexpr (PAIR)
+#pragma unroll
+                    for (int p = 0; p < NS; ++p) *reinterpret_cast<uint4*>(lz + TZ + fc_byte<T, NP>(h * 16 + r, p * KSTEP<T> + q * V)) = __builtin_bit_cast(uint4, dl[p]);
             }
         }
         if (a.want_dw) {
@@ -924,6 +980,16 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
 #pragma unroll
             for (int i = 0; i < FN; ++i) fz[i] = frag<T, false, NP, false>(lz, 0, i, 0, lane);
             mma_block<T>(dw, fz, fx);
+            if constexpr (PAIR) {
+                // the low halves' scale goes to x here: a scaled copy of the sums would cost their registers again.  x 2^-11 is exact down to 2^-3 and
+                // off by at most 2^-25, on a term that is 2^-11 of the high one.
+                if constexpr (LO_UP<T> != 1.0f)
+#pragma unroll
+                    for (int j = 0; j < FK; ++j) fx[j] *= (T)(1.0f / LO_UP<T>);
+#pragma unroll
+                for (int i = 0; i < FN; ++i) fz[i] = frag<T, false, NP, false>(lz + TZ, 0, i, 0, lane);
+                mma_block<T>(dw, fz, fx);
+            }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
@@ -976,7 +1042,7 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
 // ---- wide backward: dz = dy act'(z), and the column sums of dz -----------------------------------------------------------------------------------
 // Bound by memory: 57600 x 128 fp32 17 - 21 us = 4.2 - 5.3 TB/s (the plain products then read dz twice; forming it inside them would read dy and z as often).
 struct DzArgs {
-    const void* dy; const float* z; void* dz; float* part;
+    const void* dy; const float* z; void* dz; void* lo; float* part;      // lo: the pair's low halves (16-bit types)
     long rows, dpitch; int N, act;
     int cols, rpb; long rows_per;
 };
@@ -1001,7 +1067,16 @@ __global__ __launch_bounds__(NT) void k_dz(DzArgs a) {
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) s[i] += d[i];
-            if (a.dz) store_vec<T, V>((T*)a.dz + r * a.N + c0, d);   // the products take operands of the arrays' type: the one rounding of dz
+            if (!a.dz) continue;
+            if constexpr (sizeof(T) == 4) {
+                store_vec<T, V>((T*)a.dz + r * a.N + c0, d);
+            } else {
+                T hi[V], lo[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) dz_pair<T>(d[i] * DZ_DOWN<T>, &hi[i], &lo[i]);
+                __builtin_memcpy((T*)a.dz + r * a.N + c0, hi, sizeof hi);
+                __builtin_memcpy((T*)a.lo + r * a.N + c0, lo, sizeof lo);
+            }
         }
     }
     if (!a.part) return;
@@ -1062,8 +1137,10 @@ void join_launch(const GemmArgs& a, const float* part, long rec, int splits, int
 }
 
 // C = epilogue(A B) by tiles; ws: splits * M * N floats when splits > 1
-template <class T, bool AKC, bool BKC>
+template <class T, bool AKC, bool BKC, bool PAIR = false>
 void gemm_launch(GemmArgs a, int splits, float* ws, hipStream_t s) {
+    if constexpr (sizeof(T) == 2 && AKC == BKC && !PAIR)     // dx, dw
+        if (a.Alo || a.Blo) return gemm_launch<T, AKC, BKC, true>(a, splits, ws, s);
     GemmArgs j = a;
     a.k_per = a.K;
     if (splits > 1) {
@@ -1086,18 +1163,18 @@ void gemm_launch(GemmArgs a, int splits, float* ws, hipStream_t s) {
             return true;
         };
         static LdsConfig c128, c256;
-        if (wn == 128 && go(k_gemm_wide<T, AKC, BKC, 128>, c128)) return;
+        if (wn == 128 && go(k_gemm_wide<T, AKC, BKC, 128, PAIR>, c128)) return;
         if constexpr (sizeof(T) == 2)
-            if (wn == 256 && go(k_gemm_wide<T, AKC, BKC, 256>, c256)) return;
+            if (wn == 256 && go(k_gemm_wide<T, AKC, BKC, 256, PAIR>, c256)) return;
     }
     const int bn = bn_of(a.N), bm = bm_of(a.M, a.N);
     a.mt = (int)((a.M + bm - 1) / bm);
     a.nt = (a.N + bn - 1) / bn;
     auto go = [&](auto fn) { hipLaunchKernelGGL(fn, dim3((unsigned)(a.mt * a.nt), splits), dim3(NT), 0, s, a); };
-    if (bn == 32) go(k_gemm<T, AKC, BKC, 128, 32, 4>);
-    else if (bn == 64) go(k_gemm<T, AKC, BKC, 128, 64, 2>);
-    else if (bm == 64) go(k_gemm<T, AKC, BKC, 64, 128, 1>);
-    else go(k_gemm<T, AKC, BKC, 128, 128, 2>);
+    if (bn == 32) go(k_gemm<T, AKC, BKC, 128, 32, 4, PAIR>);
+    else if (bn == 64) go(k_gemm<T, AKC, BKC, 128, 64, 2, PAIR>);
+    else if (bm == 64) go(k_gemm<T, AKC, BKC, 64, 128, 1, PAIR>);
+    else go(k_gemm<T, AKC, BKC, 128, 128, 2, PAIR>);
     if (splits > 1) join_launch<T>(j, ws, a.M * a.N, splits, 0, nullptr, s);
 }
 
@@ -1172,8 +1249,8 @@ void dz_geometry(DzArgs& a, int V, int* blocks, int* tiles) {
     *blocks = (int)((a.rows + a.rows_per - 1) / a.rows_per);
 }
 
-// workspace of the backward pass: z (where it is formed again) | dz | column sums | partial products, each 256-byte aligned
-struct BwdWs { size_t dz, sums, part, total; int blocks, dx_splits, dw_splits; };
+// workspace of the backward pass: z (where it is formed again) | dz | its low halves (16-bit types) | column sums | partial products, each 256-byte aligned
+struct BwdWs { size_t dz, lo, sums, part, total; int blocks, dx_splits, dw_splits; };
 BwdWs linear_ws(const ttc_linear_desc* d, bool have_z) {
     const auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
     BwdWs w{};
@@ -1189,7 +1266,8 @@ BwdWs linear_ws(const ttc_linear_desc* d, bool have_z) {
     int tiles;
     dz_geometry(z, col_vec(d->cout, dtype_bytes(d->dtype)), &w.blocks, &tiles);
     w.dz = act && !have_z ? up(cells * sizeof(float)) : 0;
-    w.sums = w.dz + (act ? up(cells * dtype_bytes(d->dtype)) : 0);
+    w.lo = w.dz + (act ? up(cells * dtype_bytes(d->dtype)) : 0);
+    w.sums = w.lo + (act && d->dtype != TTC_DT_F32 ? up(cells * 2) : 0);
     w.part = w.sums + up((size_t)w.blocks * d->cout * sizeof(float));
     const size_t zs = act && !have_z ? (size_t)gemm_splits(d->rows, d->cout, d->cin, dtype_bytes(d->dtype)) : 1;
     w.dx_splits = gemm_splits(d->rows, d->cin, d->cout, dtype_bytes(d->dtype));
@@ -1233,19 +1311,34 @@ void dz_launch(const DzArgs& z, int V, int blocks, int tiles, hipStream_t s) {
 }
 
 template <class T>
-void narrow_bwd_launch(const NarrowBwd& a, int blocks, hipStream_t s) {
+hipError_t narrow_bwd_launch(const NarrowBwd& a, int blocks, hipStream_t s) {
+    auto launch = [&](auto fn, int lds, LdsConfig& cfg) {
+        if (const hipError_t e = cfg.ensure(fn, lds); e != hipSuccess) return e;
+        hipLaunchKernelGGL(fn, dim3(blocks), dim3(NT), lds, s, a);
+        return hipSuccess;
+    };
     auto go = [&](auto ks, auto ns) {
         constexpr int KS = decltype(ks)::value, NS = decltype(ns)::value;
-        if (a.K == KS * KSTEP<T> && a.N == NS * KSTEP<T> && !a.z) hipLaunchKernelGGL((k_narrow_bwd<T, KS, NS, true>), dim3(blocks), dim3(NT), 0, s, a);
-        else hipLaunchKernelGGL((k_narrow_bwd<T, KS, NS, false>), dim3(blocks), dim3(NT), 0, s, a);
+        auto pick = [&](auto pair) {
+            constexpr bool PAIR = decltype(pair)::value;
+            static LdsConfig full, ragged;
+            if (a.K == KS * KSTEP<T> && a.N == NS * KSTEP<T> && !a.z) return launch(k_narrow_bwd<T, KS, NS, true, PAIR>, NARROW_BWD_LDS<T, KS, NS, PAIR>(), full);
+            return launch(k_narrow_bwd<T, KS, NS, false, PAIR>, NARROW_BWD_LDS<T, KS, NS, PAIR>(), ragged);
+        };
+        if constexpr (sizeof(T) == 2)
+            if (a.act != TTC_ACT_NONE) return pick(std::true_type{});
+        return pick(std::false_type{});
     };
     constexpr std::integral_constant<int, 2> two{};
     constexpr std::integral_constant<int, 4> four{};
     const int half = 2 * KSTEP<T>;
-    if (a.K <= half && a.N <= half) go(two, two);
-    else if (a.K <= half) go(two, four);
-    else if (a.N <= half) go(four, two);
-    else if constexpr (sizeof(T) == 4) go(four, four);
+    if constexpr (sizeof(T) == 2)                  // a head: half the padding (898704 x 64 -> 1 sigmoid 121 us -> 70, 64 -> 32 swish 154 -> 59)
+        if (a.K <= half && a.N <= KSTEP<T>) return go(two, std::integral_constant<int, 1>{});
+    if (a.K <= half && a.N <= half) return go(two, two);
+    if (a.K <= half) return go(two, four);
+    if (a.N <= half) return go(four, two);
+    if constexpr (sizeof(T) == 4) return go(four, four);
+    return hipErrorInvalidValue;                   // narrow_bwd has no such sizes
 }
 
 }  // namespace
@@ -1325,15 +1418,16 @@ ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void*
             return TTC_OK;
         }
         char* ws = (char*)d_ws;
+        const float alpha = d->scale / (act ? DZ_DOWN<T> : 1.0f);
         GemmArgs o{};                                        // dw [cin, cout], scaled where the splits are joined
-        o.M = d->cin; o.N = d->cout; o.C = d_dw; o.ldc = d->cout; o.alpha = d->scale;
+        o.M = d->cin; o.N = d->cout; o.C = d_dw; o.ldc = d->cout; o.alpha = alpha;
         if (narrow_bwd(d)) {
             NarrowBwd a{};
             a.x = d_x; a.dy = d_dy; a.w = d_w; a.bias = d_bias; a.z = act ? d_preact : nullptr; a.dx = d_dx;
             a.part = d_dw || d_dbias ? (float*)ws : nullptr;
             a.M = d->rows; a.ldx = d->x_pitch; a.ldy = d->dy_pitch; a.ldw = d->w_pitch;
-            a.K = d->cin; a.N = d->cout; a.act = d->activation; a.scale = d->scale; a.want_dw = d_dw != nullptr; a.want_db = d_dbias != nullptr;
-            narrow_bwd_launch<T>(a, w.blocks, s);
+            a.K = d->cin; a.N = d->cout; a.act = d->activation; a.scale = alpha; a.want_dw = d_dw != nullptr; a.want_db = d_dbias != nullptr;
+            TTC_HIP(c, narrow_bwd_launch<T>(a, w.blocks, s));
             if (a.part) join_launch<T>(o, a.part, (long)d->cin * d->cout + d->cout, w.blocks, d_dbias ? d->cout : 0, d_dbias, s);
             return TTC_OK;
         }
@@ -1346,10 +1440,11 @@ ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void*
             z = (const float*)ws;
         }
         const T* dz = act ? (const T*)(ws + w.dz) : (const T*)d_dy;     // without an activation dz is dy itself; the scale is in the epilogues either way
+        const void* dz_lo = act && sizeof(T) == 2 ? ws + w.lo : nullptr;
         const long dz_pitch = act ? d->cout : d->dy_pitch;
         if (act || d_dbias) {
             DzArgs q{};
-            q.dy = d_dy; q.z = z; q.dz = act && (d_dx || d_dw) ? ws + w.dz : nullptr; q.part = d_dbias ? (float*)(ws + w.sums) : nullptr;
+            q.dy = d_dy; q.z = z; q.dz = act && (d_dx || d_dw) ? ws + w.dz : nullptr; q.lo = ws + w.lo; q.part = d_dbias ? (float*)(ws + w.sums) : nullptr;
             q.rows = d->rows; q.dpitch = d->dy_pitch; q.N = d->cout; q.act = d->activation;
             const int V = col_vec(d->cout, sizeof(T));
             int blocks, tiles;
@@ -1363,14 +1458,14 @@ ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void*
         }
         if (d_dx) {
             GemmArgs a{};
-            a.A = dz; a.lda = dz_pitch; a.B = d_w; a.ldb = d->w_pitch;
+            a.A = dz; a.Alo = dz_lo; a.lda = dz_pitch; a.B = d_w; a.ldb = d->w_pitch;
             a.M = d->rows; a.N = d->cin; a.K = d->cout;
-            a.C = d_dx; a.ldc = d->cin; a.alpha = d->scale;
+            a.C = d_dx; a.ldc = d->cin; a.alpha = alpha;
             gemm_launch<T, true, true>(a, w.dx_splits, (float*)(ws + w.part), s);
         }
         if (d_dw) {
             GemmArgs a = o;
-            a.A = d_x; a.lda = d->x_pitch; a.B = dz; a.ldb = dz_pitch; a.K = d->rows;
+            a.A = d_x; a.lda = d->x_pitch; a.B = dz; a.Blo = dz_lo; a.ldb = dz_pitch; a.K = d->rows;
             gemm_launch<T, false, false>(a, w.dw_splits, (float*)(ws + w.part), s);
         }
         return TTC_OK;

@@ -1,0 +1,67 @@
+"""GPU: the channels-last layer operators where a wrong value hides inside a wide tolerance -- gradients of 16-bit arrays held to their own final rounding.
+
+The bounds are formed as in test_gpu_layers (H, U, TINY: half a step of the result's type, 2^-24, half the spacing of fp16 subnormals)."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+from tests.test_gpu_layers import DT, H, TINY, U, act64, randn, within      # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    from ttc import _lib
+    return _lib.Context(win_in=44, length=1, max_windows=1)
+
+
+# ---- product: dz = dy act'(z) keeps more bits than the arrays' type --------------------------------------------------------------------
+
+def check_grads(dy, x, w, bias, act, scale, got):
+    """linear_backward's gradients with dz as a pair of 16-bit values: hi within H, what is left within H again (bf16 2^-16 in all, fp16 2^-22), fp16 no
+    finer than 2^-35 (half the spacing of the low half, 2^-25, is 2^-11 of its own scale, twice that for the halved value); in fp16 x as factor of the low
+    half may be off by 2^-25 against a factor of at most |dz| / 2, twice that again for the halved value"""
+    dt, h = x.dtype, H(x.dtype)
+    x2, w2, d = x.double(), w.double(), dy.double()
+    z, S = x2 @ w2 + bias.double(), x2.abs() @ w2.abs() + bias.double().abs()
+    ez = (x.shape[1] + 4) * U * S
+    _, slope = act64(z, act)
+    dz = scale * d * slope
+    e = abs(scale) * d.abs() * (0.8 * (ez + 2 * U * z.abs()) + 64 * U * z.abs().clamp(min=1) * (slope.abs() + U)) + 3 * U * dz.abs()
+    e = e + h * h * (dz.abs() + e) + (2.0 ** -35 * abs(scale) if dt == torch.float16 else 0.0)
+    dx, dw, db = got
+    n, m = w.shape[1], x.shape[0]
+    ref = dz @ w2.t()
+    b = e @ w2.abs().t() + (2 * n + 8) * U * (dz.abs() @ w2.abs().t())
+    within("dx", dx, ref, b + h * (ref.abs() + b) + TINY(dt))
+    ref = x2.t() @ dz
+    b = x2.abs().t() @ e + (2 * m + 8) * U * (x2.abs().t() @ dz.abs()) + (2.0 ** -25 * dz.abs().sum(0) if dt == torch.float16 else 0.0)
+    within("dw", dw, ref, b + h * (ref.abs() + b) + TINY(dt))
+    within("dbias", db, dz.sum(0), e.sum(0) + (m + 8) * U * dz.abs().sum(0) + U * TINY(torch.float16))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("shape", [(640, 64, 64), (700, 50, 33), (301, 40, 128), (301, 128, 40), (77, 64, 1), (900, 61, 30), (333, 64, 32), (600, 177, 93), (515, 300, 264), (300, 264, 1024),
+                                   (1024, 65, 129), (6400, 640, 128), (128, 6400, 640), (64, 2048, 2048), (2048, 2048, 64)], ids=str)
+def test_linear_gradients_are_rounded_once(ctx, dtype, shape):
+    m, k, n = shape
+    dt, act = DT[dtype], ("swish", "sigmoid", "gelu", "tanh")[(m + k + n) % 4]
+    x, w, dy, bias = randn((m, k), dt, 1), randn((k, n), dt, 2, k ** -0.5), randn((m, n), dt, 3), randn((n,), torch.float32, 4, 0.3)
+    _, pre = ctx.linear(x, w, bias, activation=act, want_preact=True)
+    for kept in {id(None): None, id(pre): pre}.values():
+        check_grads(dy, x, w, bias, act, 0.5, ctx.linear_backward(dy, x, w, kept, bias, activation=act, scale=0.5))
+
+
+@pytest.mark.parametrize("shape", [(2000, 64, 64), (2000, 60, 40), (2000, 177, 93), (128, 6400, 640)], ids=str)
+def test_linear_fp16_slopes_below_and_above_the_types_range(ctx, shape):
+    m, k, n = shape
+    # dy act' about 1e-7, below fp16's smallest normal value: sums over many rows are not
+    x, w, dy = randn((m, k), torch.float16, 1, 8.0), randn((k, n), torch.float16, 2, 0.02 * k ** -0.5), randn((m, n), torch.float16, 3, 1e-3)
+    bias = randn((n,), torch.float32, 4, 0.3, 9.0)
+    _, pre = ctx.linear(x, w, bias, activation="sigmoid", want_preact=True)
+    check_grads(dy, x, w, bias, "sigmoid", 1.0, ctx.linear_backward(dy, x, w, pre, bias, activation="sigmoid"))
+    # dy act' past its largest value, gradients well inside
+    x, w = randn((m, k), torch.float16, 5, 1e-4), randn((k, n), torch.float16, 6, 1e-3)
+    bias, dy = torch.full((n,), 1.4, device="cuda"), torch.full((m, n), 64000.0, device="cuda", dtype=torch.float16)
+    _, pre = ctx.linear(x, w, bias, activation="gelu", want_preact=True)
+    check_grads(dy, x, w, bias, "gelu", 1.0, ctx.linear_backward(dy, x, w, pre, bias, activation="gelu"))
