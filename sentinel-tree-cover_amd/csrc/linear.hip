@@ -898,8 +898,12 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
 #pragma unroll
                     for (int i = 0; i < V; ++i) { t[i] = (float)dv[i]; zz[i] = z[H16 ? 2 * p + i / 4 : p][0][i & 3]; }
                     slope_vec<V>(t, zz, a.act);
+                    int cols = FULL ? V : a.N - p * KSTEP<T> - q * V;
+                    if (!FULL) asm volatile("" : "+v"(cols));           // compared where it is used: as masks kept over the loop it is 16 registers
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
+                        // a padded column: its zero weights make z NaN where x is infinite, and that times its zero dy would reach every dx of the row
+                        if (!FULL && i >= cols) t[i] = 0.0f;
                         t[i] *= DZ_DOWN<T>;
                         db[p][i] += t[i];
                         if constexpr (PAIR) {

@@ -65,3 +65,53 @@ def test_linear_fp16_slopes_below_and_above_the_types_range(ctx, shape):
     bias, dy = torch.full((n,), 1.4, device="cuda"), torch.full((m, n), 64000.0, device="cuda", dtype=torch.float16)
     _, pre = ctx.linear(x, w, bias, activation="gelu", want_preact=True)
     check_grads(dy, x, w, bias, "gelu", 1.0, ctx.linear_backward(dy, x, w, pre, bias, activation="gelu"))
+
+
+# ---- infinities and NaN in the backward passes -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("act", ["relu", "sigmoid", "tanh"])
+def test_linear_gradients_of_rows_with_infinities_and_nan(ctx, dtype, act):
+    """an infinite x has an infinite argument and a slope of 0 or 1: that row's dx is finite, at widths with and without padded columns alike; a NaN stays in
+    its row, and neither reaches another row"""
+    dt = DT[dtype]
+    for m, k, n in ((100, 64, 64), (100, 64, 1), (100, 64, 20), (101, 50, 33), (70, 33, 63), (90, 64, 128), (90, 128, 50), (150, 200, 150), (2, 64, 5)):
+        x, w, dy = randn((m, k), dt, 1), randn((k, n), dt, 2, k ** -0.5), randn((m, n), dt, 3)
+        w = torch.where(w == 0, torch.ones_like(w), w)
+        bias = randn((n,), torch.float32, 4, 0.3)
+        bad = x.clone()
+        rows = {0: float("inf"), m - 1: float("nan")} if m < 50 else {3: float("inf"), 17: float("-inf"), m - 1: float("inf"), 40: float("nan")}
+        for r, v in rows.items():
+            bad[r, (7 * r) % k] = v
+        pre = bad.double() @ w.double() + bias.double()
+        dx0, _, _ = ctx.linear_backward(dy, x, w, None, bias, activation=act)
+        for kept in (None, pre.float()):
+            dx, dw, db = ctx.linear_backward(dy, bad, w, kept, bias, activation=act)
+            slope = {"relu": (pre > 0).double(), "sigmoid": torch.zeros_like(pre), "tanh": torch.zeros_like(pre)}[act]
+            for r, v in rows.items():
+                if v != v:
+                    assert bool(dx[r].isnan().all()), (m, k, n, r)
+                    continue
+                assert bool(pre[r].isinf().all())
+                dz = dy[r].double() * slope[r]
+                ref, mag = dz @ w.double().t(), dz.abs() @ w.double().abs().t()
+                within(f"dx of row {r} of {(m, k, n)}", dx[r], ref, (n + 8) * U * mag + H(dt) * (ref.abs() + (n + 8) * U * mag) + TINY(dt))
+            if kept is None:
+                others = [r for r in range(m) if r not in rows]
+                assert torch.equal(dx[others], dx0[others])
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("rows", [50, 40000])
+def test_group_norm_gradients_of_a_group_with_nan(ctx, dtype, rows):
+    """NaN and infinities stay in their sample's group, and in the parameter gradients of its channels: one launch and several"""
+    dt = DT[dtype]
+    x, dy, gamma = randn((3, rows, 16), dt, 1), randn((3, rows, 16), dt, 2), randn((16,), torch.float32, 3)
+    for v in (float("nan"), float("inf")):
+        bad = x.clone()
+        bad[1, 7, 5] = v
+        _, st = ctx.group_norm(bad, gamma, None, groups=4, activation="tanh", want_stats=True)
+        dx, dg, db = ctx.group_norm_backward(dy, bad, gamma, None, st, activation="tanh")
+        assert bool(dx[1, :, 4:8].isnan().all()) and bool(dg[4:8].isnan().all()) and bool(db[4:8].isnan().all())
+        dx[1, :, 4:8], dg[4:8], db[4:8] = 0, 0, 0
+        assert bool(dx.isfinite().all()) and bool(dg.isfinite().all()) and bool(db.isfinite().all())
