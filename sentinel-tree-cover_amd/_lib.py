@@ -921,6 +921,15 @@ class Context:
             raise ValueError(f"{what} must be [{c}], got {tuple(p.shape)}")
         return p if p.dtype is self.torch.float32 and p.is_contiguous() else p.detach().to(self.torch.float32).contiguous()
 
+    def _layer_number(self, v, what, kind=float):
+        """a plain number: plans are looked up by it, and a tensor would be found by its identity whatever it holds by then"""
+        if isinstance(v, self.torch.Tensor) and v.requires_grad and self.torch.is_grad_enabled():
+            raise ValueError(f"{what} is a constant of the call: no gradient flows into it (pass a number, or detach it)")
+        n = kind(v)
+        if kind is int and n != v:
+            raise ValueError(f"{what} must be a whole number, got {v}")
+        return n
+
     def _layer_plan(self, key, make):
         plans = self.__dict__.setdefault("_plans", {})
         plan = plans.get(key)
@@ -953,6 +962,7 @@ class Context:
         want_stats: also the float32 [n, groups, 2] (mean, 1 / sqrt(var + eps)) that group_norm_backward takes.  Differentiable in x, gamma and
         beta through torch.autograd (want_stats False)."""
         x, gamma, beta = self._layer_arg(x, "group_norm: x"), self._layer_arg(gamma, "group_norm: gamma"), self._layer_arg(beta, "group_norm: beta")
+        groups, eps = self._layer_number(groups, "group_norm: groups", int), self._layer_number(eps, "group_norm: eps")
         if self._wants_grad("group_norm", x, gamma, beta):
             if want_stats:
                 raise ValueError("group_norm: want_stats is for calls without autograd (under torch.no_grad())")
@@ -968,7 +978,7 @@ class Context:
         n, c = x.shape[0], x.shape[-1]
         v, sn, pitch = _rows(x, 1)
         rows = x.numel() // (n * c) if n and c else 0
-        d = TTCGroupNormDesc(code, act, n, rows, c, int(groups), sn, pitch, float(eps))
+        d = TTCGroupNormDesc(code, act, n, rows, c, groups, sn, pitch, eps)
         return d, C.byref(d), v is not x, self._layer_ws(self.lib.ttc_group_norm_workspace, d, backward), c
 
     def _group_norm(self, x, gamma, beta, groups, eps, activation, want_stats):
@@ -1029,6 +1039,7 @@ class Context:
         Differentiable in x, w, bias and residual through torch.autograd (want_preact False)."""
         x, w, bias, residual = (self._layer_arg(x, "linear: x"), self._layer_arg(w, "linear: w"), self._layer_arg(bias, "linear: bias"),
                                 self._layer_arg(residual, "linear: residual"))
+        scale = self._layer_number(scale, "linear: scale")
         if self._wants_grad("linear", x, w, bias, residual):
             if want_preact:
                 raise ValueError("linear: want_preact is for calls without autograd (under torch.no_grad())")
@@ -1048,7 +1059,7 @@ class Context:
         wcopy = (cout > 1 and w.stride(1) != 1) or (cin > 1 and w.stride(0) < cout)
         v, _, pitch = _rows(x, 0)
         rows = x.numel() // cin if cin else 0
-        d = TTCLinearDesc(code, act, rows, cin, cout, pitch, cout if wcopy or cin <= 1 else w.stride(0), cout, cout, float(scale))
+        d = TTCLinearDesc(code, act, rows, cin, cout, pitch, cout if wcopy or cin <= 1 else w.stride(0), cout, cout, scale)
         return d, v is not x, wcopy, tuple(x.shape[:-1]) + (cout,)
 
     def _linear(self, x, w, bias, residual, activation, scale, want_preact):
@@ -1088,6 +1099,7 @@ class Context:
         t = self.torch
         what = "linear_backward"
         dy, x, w, preact, bias = (self._layer_arg(a, f"{what}: {k}") for a, k in ((dy, "dy"), (x, "x"), (w, "w"), (preact, "preact"), (bias, "bias")))
+        scale = self._layer_number(scale, what + ": scale")
 
         def make():
             d, copy, wcopy, shape = self._linear_desc(x, w, activation, scale, what)

@@ -124,3 +124,44 @@ def test_plans_are_kept_by_shape_alone_and_bounded(host):
     n = len(made)
     host._layer_plan(("k", 4999), lambda: made.append(0))
     assert len(made) == n
+
+
+class Recorder:
+    """the library with its layer entries replaced by ones that note their descriptors: the binding's own work, without a device"""
+    def __init__(self, lib):
+        self.lib, self.calls = lib, []
+
+    def __getattr__(self, name):
+        if name in ("ttc_linear", "ttc_linear_backward", "ttc_group_norm", "ttc_group_norm_backward"):
+            return lambda h, ref, *rest: self.calls.append((name, ref._obj, rest)) or 0
+        return getattr(self.lib, name)
+
+
+@pytest.fixture
+def recorded(lib, host):
+    host.lib, host.device, host._layer_stream = Recorder(lib), -1, lambda: 0       # tensors of the CPU are device -1
+    return host
+
+
+def test_numbers_given_as_tensors_are_read_at_every_call(recorded):
+    x, w, dy, s = torch.zeros(4, 16), torch.zeros(16, 8), torch.zeros(4, 8), torch.tensor(0.5)
+    for v in (0.5, 2.0):
+        s.fill_(v)
+        recorded.linear(x, w, scale=s)
+        recorded.linear_backward(dy, x, w, scale=s)
+        recorded.group_norm(x, groups=4, eps=s)
+    assert [getattr(d, "scale", None) or d.eps for _, d, _ in recorded.lib.calls] == [0.5] * 3 + [2.0] * 3
+    g = torch.tensor(4)
+    for v in (4, 8):
+        g.fill_(v)
+        recorded.group_norm(x, groups=g)
+        assert recorded.lib.calls[-1][1].groups == v
+    with pytest.raises(ValueError, match="groups must be a whole number"):
+        recorded.group_norm(x, groups=2.5)
+    p = torch.tensor(1.0, requires_grad=True)
+    for call in (lambda: recorded.linear(x, w, scale=p), lambda: recorded.linear_backward(dy, x, w, scale=p), lambda: recorded.group_norm(x, groups=4, eps=p)):
+        with pytest.raises(ValueError, match="no gradient flows"):
+            call()
+    with torch.no_grad():
+        recorded.linear(x, w, scale=p)
+    assert recorded.lib.calls[-1][1].scale == 1.0
