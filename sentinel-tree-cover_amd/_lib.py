@@ -947,8 +947,15 @@ class Context:
     def _layer_stream(self):
         return self.torch._C._cuda_getCurrentRawStream(self.device)
 
+    def _no_tangents(self, what, *tensors):
+        """forward-mode differentiation has no rule here: a tangent must not get lost in silence"""
+        fw = self.torch.autograd.forward_ad
+        if fw._current_level >= 0 and any(a is not None and fw.unpack_dual(a).tangent is not None for a in tensors):
+            raise RuntimeError(f"{what}: forward-mode differentiation is not supported")
+
     def _wants_grad(self, what, *tensors):
         t = self.torch
+        self._no_tangents(what, *tensors)
         if not t.is_grad_enabled() or not any(a is not None and a.requires_grad for a in tensors):
             return False
         if t.cuda.is_current_stream_capturing():
@@ -1006,6 +1013,7 @@ class Context:
         t = self.torch
         what = "group_norm_backward"
         dy, x, gamma, beta, stats = (self._layer_arg(a, f"{what}: {k}") for a, k in ((dy, "dy"), (x, "x"), (gamma, "gamma"), (beta, "beta"), (stats, "stats")))
+        self._no_tangents(what, dy, x, gamma, beta, stats)
         if stats.dim() != 3 or stats.shape[2] != 2 or stats.shape[0] != x.shape[0] or stats.dtype != t.float32:
             raise ValueError(f"{what}: stats must be the float32 [{x.shape[0]}, groups, 2] of the forward call, got {stats.dtype} {tuple(stats.shape)}")
         if dy.shape != x.shape or dy.dtype != x.dtype:
@@ -1099,6 +1107,7 @@ class Context:
         t = self.torch
         what = "linear_backward"
         dy, x, w, preact, bias = (self._layer_arg(a, f"{what}: {k}") for a, k in ((dy, "dy"), (x, "x"), (w, "w"), (preact, "preact"), (bias, "bias")))
+        self._no_tangents(what, dy, x, w, preact, bias)
         scale = self._layer_number(scale, what + ": scale")
 
         def make():

@@ -165,3 +165,20 @@ def test_numbers_given_as_tensors_are_read_at_every_call(recorded):
     with torch.no_grad():
         recorded.linear(x, w, scale=p)
     assert recorded.lib.calls[-1][1].scale == 1.0
+
+
+def test_forward_mode_tangents_are_refused(recorded):
+    import torch.autograd.forward_ad as fw
+    x, w, dy, g, st = torch.zeros(4, 16), torch.zeros(16, 8), torch.zeros(4, 8), torch.ones(16), torch.zeros(4, 4, 2)
+    with fw.dual_level():
+        dual = lambda a: fw.make_dual(a, torch.ones_like(a))      # noqa: E731
+        for call in (lambda: recorded.linear(dual(x), w), lambda: recorded.linear(x, dual(w)), lambda: recorded.linear(x, w, residual=dual(dy)),
+                     lambda: recorded.linear(x, w, bias=dual(torch.zeros(8))), lambda: recorded.group_norm(dual(x), groups=4),
+                     lambda: recorded.group_norm(x, g, dual(g), groups=4), lambda: recorded.linear_backward(dual(dy), x, w),
+                     lambda: recorded.group_norm_backward(x, x, dual(g), None, st)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert not recorded.lib.calls
+        recorded.linear(x, w)                                     # no tangent: an ordinary call
+        recorded.group_norm_backward(x, x, g, None, st)
+    assert len(recorded.lib.calls) == 2
