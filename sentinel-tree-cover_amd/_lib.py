@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import warnings
 
 import numpy as np
 
@@ -82,6 +83,7 @@ class TTCLinearDesc(C.Structure):
                 ("x_pitch", C.c_int64), ("w_pitch", C.c_int64), ("res_pitch", C.c_int64), ("dy_pitch", C.c_int64), ("scale", C.c_float)]
 
 
+_OMITTED = object()                      # default of linear_backward's bias: not the same as a layer without one (None)
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "swish": 2, "sigmoid": 3, "tanh": 4, "gelu": 5}     # TTC_ACT_*
 
 
@@ -1100,12 +1102,18 @@ class Context:
                                         ws.data_ptr() if nb else None, nb, self._layer_stream()), "ttc_linear")
         return y, preact
 
-    def linear_backward(self, dy, x, w, preact=None, bias=None, activation=None, scale=1.0, want_dx=True, want_dw=True, want_dbias=True):
+    def linear_backward(self, dy, x, w, preact=None, bias=_OMITTED, activation=None, scale=1.0, want_dx=True, want_dw=True, want_dbias=True):
         """ttc_linear_backward: gradients of linear(x, w, bias, residual, activation, scale) for dy [..., cout] -> (dx, dw, dbias), None where not wanted;
-        dbias float32 [cout].  The residual's gradient is dy.  `preact` as linear(..., want_preact=True) returned it; without it an activation's argument is
-        formed again from x, w and the forward call's bias."""
+        dbias float32 [cout].  The residual's gradient is dy.  `preact` as linear(..., want_preact=True) returned it; where that is None an activation's argument
+        is formed again from x, w and the forward call's bias, so pass both: which of the two is read depends on the layer's size (bias=None: a layer
+        without one; left out where it would be read, the call warns)."""
         t = self.torch
         what = "linear_backward"
+        if bias is _OMITTED:
+            bias = None
+            if preact is None and ACTIVATIONS.get(activation):
+                warnings.warn(f"{what}: neither preact nor bias was given, so the argument of {activation} is formed without a bias: pass the forward call's "
+                              "bias (bias=None if it had none)", stacklevel=2)
         dy, x, w, preact, bias = (self._layer_arg(a, f"{what}: {k}") for a, k in ((dy, "dy"), (x, "x"), (w, "w"), (preact, "preact"), (bias, "bias")))
         self._no_tangents(what, dy, x, w, preact, bias)
         scale = self._layer_number(scale, what + ": scale")

@@ -182,3 +182,21 @@ def test_forward_mode_tangents_are_refused(recorded):
         recorded.linear(x, w)                                     # no tangent: an ordinary call
         recorded.group_norm_backward(x, x, g, None, st)
     assert len(recorded.lib.calls) == 2
+
+
+def test_a_left_out_bias_is_noticed_where_it_would_be_read(recorded):
+    import warnings
+    for cin, cout in ((16, 8), (16, 300)):                        # narrow: formed again from x, w and bias; wide: the kept preact
+        x, w, dy, bias = torch.zeros(4, cin), torch.zeros(cin, cout), torch.zeros(4, cout), torch.zeros(cout)
+        _, pre = recorded.linear(x, w, bias, activation="swish", want_preact=True)
+        assert (pre is None) == (cout == 8)
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            recorded.linear_backward(dy, x, w, pre, bias, activation="swish")
+            recorded.linear_backward(dy, x, w, None, None, activation="swish")          # a layer without one
+            recorded.linear_backward(dy, x, w)                                          # no activation: nothing to form
+            if pre is not None:
+                recorded.linear_backward(dy, x, w, pre, activation="swish")
+                continue
+        with pytest.warns(UserWarning, match="pass the forward call's bias"):
+            recorded.linear_backward(dy, x, w, pre, activation="swish")
