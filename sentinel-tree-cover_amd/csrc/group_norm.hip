@@ -13,7 +13,7 @@
 // last-level cache, measured slower: 36 x 172 x 172 x 64 fp32 in three parts 172 us against 154.)
 // A thread owns one vector of channels (up to 16 bytes) and walks rows: the inner loop knows no groups, and a row is read as whole cache lines.
 // Numerics: a thread sums (x - x0) and (x - x0)^2 about its own first row in 32 bits, folds into 64-bit sums every 128 values; the forward sums across
-// threads are 64-bit, the backward ones 32-bit trees of at most a few thousand rows joined in 64 bits; the order is fixed (no atomics).
+// threads are 64-bit, the backward ones 32-bit runs of at most 512 rows (a resident sample: 32-bit trees) joined in 64 bits; the order is fixed (no atomics).
 #include <algorithm>
 
 #include "layers_common.h"
@@ -25,6 +25,7 @@ constexpr int NT = 256;             // threads of the streaming kernels
 constexpr int RT = 1024, RU = 4;    // threads and vectors per thread of the resident ones
 constexpr int SU = 8;                   // loads of the forward sums in flight
 constexpr int FOLD = 128;           // values summed in 32 bits before they are folded into the 64-bit sums
+constexpr int RUN = 512;            // rows a thread of the backward sums adds in 32 bits: longer ones get more splits
 
 struct NormArgs {
     const void* x; const void* dy;
@@ -297,10 +298,10 @@ __global__ __launch_bounds__(RT) void k_gn_bwd_mid(NormArgs a) {
     const float* p = a.cpart + n * a.splits * (long)w;
     for (int i = threadIdx.x; i < w * lanes; i += RT) {
         const int c = i % w;
-        float t = 0.0f;
+        double t = 0.0;
 #pragma unroll 4
         for (int k = i / w; k < a.splits; k += lanes) t += p[(long)k * w + c];
-        sm2[i] = t;
+        sm2[i] = (float)t;
     }
     __syncthreads();
     for (int c = threadIdx.x; c < w; c += RT) {
@@ -581,15 +582,16 @@ int norm_vec(int c, int bytes) {
     return v;
 }
 
-// streaming kernels: 1024 blocks of 4 waves; a split keeps at least 4 steps of rows so that its prologue stays small
-void norm_geometry(NormArgs& a, int V) {
+// streaming kernels: 1024 blocks of 4 waves; a split keeps at least 4 steps of rows so that its prologue stays small, and backward at most RUN of them
+void norm_geometry(NormArgs& a, int V, bool backward) {
     const int cv = a.C / V;
     a.cols = std::min(cv, NT);
     a.rpb = NT / a.cols;
     a.ctiles = (cv + a.cols - 1) / a.cols;
     const long want = std::max<long>(1, 1024 / std::max<long>(1, (long)a.n * a.ctiles));
     const long most = std::max<long>(1, a.rows / (4L * a.rpb));
-    a.splits = (int)std::min<long>({want, most, 65535});
+    const long least = backward ? (a.rows + (long)RUN * a.rpb - 1) / ((long)RUN * a.rpb) : 1;
+    a.splits = (int)std::min<long>(std::max(least, std::min(want, most)), 65535);
     a.rows_per = std::max<long>(1, (a.rows + a.splits - 1) / a.splits);
     a.splits = (int)((a.rows + a.rows_per - 1) / a.rows_per);
 }
@@ -666,7 +668,7 @@ NormPlan norm_plan(const ttc_group_norm_desc* d, bool backward) {
     p.resident = d->rows > 0 && norm_resident(a, bytes, backward, &p.slab);
     if (!p.resident) {
         p.V = norm_vec(a.C, bytes);
-        norm_geometry(a, p.V);
+        norm_geometry(a, p.V, backward);
     }
     p.ws = norm_ws(a, backward, p.resident);
     return p;

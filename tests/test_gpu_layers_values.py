@@ -115,3 +115,23 @@ def test_group_norm_gradients_of_a_group_with_nan(ctx, dtype, rows):
         assert bool(dx[1, :, 4:8].isnan().all()) and bool(dg[4:8].isnan().all()) and bool(db[4:8].isnan().all())
         dx[1, :, 4:8], dg[4:8], db[4:8] = 0, 0, 0
         assert bool(dx.isfinite().all()) and bool(dg.isfinite().all()) and bool(db.isfinite().all())
+
+
+# ---- group norm: sums over many rows ---------------------------------------------------------------------------------------------------
+
+def test_group_norm_gradients_of_many_samples_of_many_rows(ctx):
+    """one large dy and 16383 small ones per channel: a 32-bit run of all rows drops every small one (2^14 + 2^-11 is 2^14 there).  513 samples, the number
+    from which their count alone fills the chip; they are one sample read 513 times (sample stride 0)"""
+    n, rows, c = 513, 16384, 2048
+    dy = torch.full((1, rows, c), 2.0 ** -11, device="cuda", dtype=torch.float16)
+    dy[:, 0] = 2.0 ** 14
+    x = torch.ones((1, rows, c), device="cuda", dtype=torch.float16)
+    x[:, 1::2] = -1.0                                             # mean 0, variance 1
+    st = torch.zeros((n, 8, 2), device="cuda")
+    st[..., 1] = (1 + 1e-5) ** -0.5
+    dx, dg, db = ctx.group_norm_backward(dy.expand(n, rows, c), x.expand(n, rows, c), None, None, st, want_dx=False)
+    assert dx is None
+    d = dy[0].double()
+    tol = (512 + 16) * U * n * d.abs().sum(0)                     # runs of 512 rows in any order; everything joined is in 64 bits
+    within("dbeta", db, n * d.sum(0), tol)
+    within("dgamma", dg, n * float(st[0, 0, 1]) * (d * x[0].double()).sum(0), tol)
