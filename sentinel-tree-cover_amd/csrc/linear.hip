@@ -1098,8 +1098,7 @@ __global__ __launch_bounds__(NT) void k_dz(DzArgs a) {
 }
 template <class T>
 __global__ void k_fill0(T* p, long n) {
-    const long i = (long)blockIdx.x * NT + threadIdx.x;
-    if (i < n) p[i] = (T)0.0f;
+    for (long i = (long)blockIdx.x * NT + threadIdx.x; i < n; i += (long)gridDim.x * NT) p[i] = (T)0.0f;
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------------
@@ -1417,7 +1416,8 @@ ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void*
         using T = decltype(tag);
         if (d->rows == 0) {
             const long n = (long)d->cin * d->cout;
-            if (d_dw) hipLaunchKernelGGL((k_fill0<T>), dim3((unsigned)((n + NT - 1) / NT)), dim3(NT), 0, s, (T*)d_dw, n);
+            // at most 2^16 workgroups: a launch is limited to 2^32 threads, and dw may have as many elements
+            if (d_dw) hipLaunchKernelGGL((k_fill0<T>), dim3((unsigned)std::min<long>((n + NT - 1) / NT, 1 << 16)), dim3(NT), 0, s, (T*)d_dw, n);
             if (d_dbias) hipLaunchKernelGGL((k_fill0<float>), dim3((d->cout + NT - 1) / NT), dim3(NT), 0, s, d_dbias, (long)d->cout);
             return TTC_OK;
         }

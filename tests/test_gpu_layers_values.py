@@ -135,3 +135,13 @@ def test_group_norm_gradients_of_many_samples_of_many_rows(ctx):
     tol = (512 + 16) * U * n * d.abs().sum(0)                     # runs of 512 rows in any order; everything joined is in 64 bits
     within("dbeta", db, n * d.sum(0), tol)
     within("dgamma", dg, n * float(st[0, 0, 1]) * (d * x[0].double()).sum(0), tol)
+
+
+# ---- the ends of the sizes -------------------------------------------------------------------------------------------------------------
+
+def test_linear_gradient_of_no_rows_at_the_largest_weights(ctx):
+    w = torch.empty((65536, 65536), device="cuda", dtype=torch.bfloat16)
+    x = torch.empty((0, 65536), device="cuda", dtype=torch.bfloat16)
+    dx, dw, db = ctx.linear_backward(x, x, w, None, None)
+    assert dx.shape == x.shape and dw.shape == w.shape and not db.any()
+    assert not any(bool(part.any()) for part in dw.split(8192))
