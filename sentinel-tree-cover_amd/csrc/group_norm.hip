@@ -601,9 +601,11 @@ void norm_geometry(NormArgs& a, int V, bool backward) {
 //  - forward: a slab's pieces of a row below 64 bytes, of more than 4 MB in all (lines fetched by several XCDs).  us resident / streaming: fp16 5 x 2867 x 40
 //    in groups of 8 8.3 / 10.2, 16 x 2867 x 64 15.4 / 11.3; fp32 8 x 1200 x 64 6.3 / 8.9, 8 x 2048 x 64 8.0 / 8.3, 32 x 2048 x 64 18.5 / 13.0, 32 x 784 x 64
 //    (64 bytes) 6.0 / 9.9.
-//  - backward: more than 13 elements a thread or a second round of workgroups (its phases wait for each other; streaming spreads them over the chip):
-//    fp16 1 x 196 x 64 9.3 / 12.9, 1 x 784 x 64 13.4 / 12.6, 5 x 2867 x 40 16.8 / 13.8, 36 x 1600 x 256 74.5 / 35.7; fp32 1 x 400 x 64 6.8 / 10.5,
-//    8 x 784 x 256 11.9 / 14.4, 32 x 2048 x 64 37.7 / 19.7, 1024 x 49 x 64 42.5 / 30.9.
+//  - backward: a second round of workgroups (its phases wait for each other; streaming spreads them over the chip: fp16 36 x 1600 x 256 74.5 / 35.7, fp32
+//    32 x 2048 x 64 37.7 / 19.7, 1024 x 49 x 64 42.5 / 30.9), and for 16-bit types more than 15 elements a thread (fp32 holds 16 at most).  Mean of resident /
+//    streaming over 1, 8 and 32 samples of 64, 128 and 256 channels in 8 groups, by elements a thread: 16-bit 8: 0.94, 12: 0.98, 14: 0.96, 16: 1.01, 20: 1.04,
+//    24: 1.07, 32: 1.12 (a few samples are over it from 8 on, 32 of 256 channels below it at 32); fp32 8: 0.88, 12: 0.91, 16: 0.95.  E.g. fp16 1 x 512 x 64
+//    12.5 / 12.6, 8 x 512 x 128 15.5 / 15.2, 32 x 512 x 256 21.2 / 24.8; fp32 1 x 1024 x 64 9.5 / 10.4, 8 x 1024 x 64 11.7 / 11.0, 32 x 512 x 256 18.1 / 24.2.
 struct Slab { int v, threads, slabs; };
 bool norm_resident(NormArgs& a, int bytes, bool backward, Slab* s) {
     s->v = norm_vec(a.cpg, bytes);
@@ -621,7 +623,7 @@ bool norm_resident(NormArgs& a, int bytes, bool backward, Slab* s) {
     s->threads = (a.cols * a.rpb + 63) / 64 * 64;
     s->slabs = (a.G + groups - 1) / groups;
     const long piece = (long)groups * a.cpg;
-    if (backward) return a.rows * piece <= 13 * RT && (long)a.n * s->slabs <= 256;
+    if (backward) return (bytes == 4 || a.rows * piece <= 15 * RT) && (long)a.n * s->slabs <= 256;
     return s->slabs == 1 || piece * bytes >= 64 || a.n * a.rows * a.C * bytes <= 4 << 20;
 }
 

@@ -6,7 +6,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from tests.test_gpu_layers import DT, H, TINY, U, act64, randn, within      # noqa: E402
+from tests.test_gpu_layers import DT, H, TINY, U, act64, check_norm, randn, within      # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -145,3 +145,13 @@ def test_linear_gradient_of_no_rows_at_the_largest_weights(ctx):
     dx, dw, db = ctx.linear_backward(x, x, w, None, None)
     assert dx.shape == x.shape and dw.shape == w.shape and not db.any()
     assert not any(bool(part.any()) for part in dw.split(8192))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(32, 784, 64, 8), (32, 841, 64, 8), (32, 961, 64, 8), (32, 1024, 64, 8), (32, 1025, 64, 8), (8, 480, 128, 8), (8, 481, 128, 8),
+                                   (1, 500, 64, 8), (257, 16, 64, 8)], ids=str)
+def test_group_norm_both_sides_of_one_launch(ctx, dtype, shape):
+    """sizes next to the ones from which a sample is no longer held by one workgroup"""
+    n, r, c, G = shape
+    x, gamma, beta = randn((n, r, c), DT[dtype], 1, 1.5, 0.7), randn((c,), torch.float32, 2, 0.3, 1.0), randn((c,), torch.float32, 3, 0.3)
+    check_norm(ctx, x, gamma, beta, G, "swish", dy=randn((n, r, c), DT[dtype], 4))
