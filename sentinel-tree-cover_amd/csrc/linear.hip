@@ -261,9 +261,7 @@ __device__ __forceinline__ void finish(const GemmArgs& a, long row, int col, int
 }
 template <class T, int V>
 __device__ __forceinline__ void emit(const GemmArgs& a, long row, int col, int left, float (&v)[V]) {
-    if (a.partial) {
-        store_part<float, V>((float*)a.C + ((long)blockIdx.y * a.M + row) * a.N + col, left, v);
-    } else if (!a.fwd) {
+    if (!a.fwd) {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] *= a.alpha;
         store_part<T, V>((T*)a.C + row * a.ldc + col, left, v);
@@ -792,7 +790,7 @@ __global__ __launch_bounds__(NT) void k_narrow(GemmArgs a) {
 struct NarrowBwd {
     const void* x; const void* dy; const void* w; const float* bias; const float* z; void* dx; float* part;
     long M, ldx, ldy, ldw; int K, N, act; float scale;
-    int want_dw, want_db;
+    int want_dw;
 };
 // image of w | per wave a tile of x, one of dz, of a pair one of the low halves | bias; at the end the sums of all four waves
 template <class T, int KS, int NS, bool PAIR>
@@ -1207,7 +1205,7 @@ void narrow_launch_k(const GemmArgs& a, hipStream_t s) {
     if (a.N <= 16) go(std::integral_constant<int, 1>{});
     else if (a.N <= 32) go(std::integral_constant<int, 2>{});
     else if (a.N <= 64) go(std::integral_constant<int, 4>{});
-    else go(std::integral_constant<int, 8>{});
+    else if constexpr (KS < 8) go(std::integral_constant<int, 8>{});         // weights of at most 32 KB
 }
 template <class T>
 void narrow_launch(const GemmArgs& a, hipStream_t s) {
@@ -1430,7 +1428,7 @@ ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void*
             a.x = d_x; a.dy = d_dy; a.w = d_w; a.bias = d_bias; a.z = act ? d_preact : nullptr; a.dx = d_dx;
             a.part = d_dw || d_dbias ? (float*)ws : nullptr;
             a.M = d->rows; a.ldx = d->x_pitch; a.ldy = d->dy_pitch; a.ldw = d->w_pitch;
-            a.K = d->cin; a.N = d->cout; a.act = d->activation; a.scale = alpha; a.want_dw = d_dw != nullptr; a.want_db = d_dbias != nullptr;
+            a.K = d->cin; a.N = d->cout; a.act = d->activation; a.scale = alpha; a.want_dw = d_dw != nullptr;
             TTC_HIP(c, narrow_bwd_launch<T>(a, w.blocks, s));
             if (a.part) join_launch<T>(o, a.part, (long)d->cin * d->cout + d->cout, w.blocks, d_dbias ? d->cout : 0, d_dbias, s);
             return TTC_OK;
