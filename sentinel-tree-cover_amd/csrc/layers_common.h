@@ -31,7 +31,7 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
 
 // exp(-v) overflows to +inf for v < -88 and 1 / inf is 0: the limits come out without a branch.  v_rcp_f32 is within 1 ulp.
 __device__ __forceinline__ float sigmoidf(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
-// 1 - 2 / (1 + e^2v) cancels near 0 (absolute error 1e-7): below 1/2 the odd Taylor series to v^13 (next term 6e-8 of v at 1/2) keeps the
+// 1 - 2 / (1 + e^2v) cancels near 0 (absolute error 1e-7): below 1/2 the odd Taylor series to v^15 (next term 9e-9 of v at 1/2) keeps the
 // relative accuracy.  Coefficients: 2^2k (2^2k - 1) B_2k / (2k)!.
 __device__ __forceinline__ float tanh_rel(float v) {
     const float t = v * v;
@@ -42,8 +42,8 @@ __device__ __forceinline__ float tanh_rel(float v) {
 }
 
 // h = normal distribution function of -|z|, and e = exp(-z^2 / 2).  h = erfc(x) / 2 with x = |z| / sqrt 2, and erfc(x) = exp(-x^2) t P(t),
-// t = 1 / (1 + 0.356 x): P is the degree-9 Chebyshev fit of exp(x^2) erfc(x) / t over t in (0, 1], 2.7e-8 of its value everywhere (0.356 minimises
-// that; P is halved below).  No 1 + erf: the negative tail keeps its relative accuracy.  A quarter of the registers of the library's erfc, which set
+// t = 1 / (1 + 0.356 x): P is the degree-9 Chebyshev fit of exp(x^2) erfc(x) / t over t in (0, 1] (0.356 minimises its error; P is halved below):
+// with the rounded coefficients within 4e-8 of its value everywhere.  No 1 + erf: the negative tail keeps its relative accuracy.  A quarter of the registers of the library's erfc, which set
 // the kernels' occupancy.
 __device__ __forceinline__ float normal_tail(float z, float* e) {
     const float az = fabsf(z), t = __builtin_amdgcn_rcpf(1.0f + (0.356f * 0.70710678f) * az);

@@ -200,3 +200,23 @@ def test_a_left_out_bias_is_noticed_where_it_would_be_read(recorded):
                 continue
         with pytest.warns(UserWarning, match="pass the forward call's bias"):
             recorded.linear_backward(dy, x, w, pre, activation="swish")
+
+
+def test_stated_errors_of_the_polynomials():
+    """the tanh series and the normal tail's fit, with the coefficients of the header, in float64 against their functions"""
+    import math
+    import os
+    import re
+    import numpy as np
+    from scipy.special import erfcx
+    text = open(os.path.join(os.path.dirname(_lib.__file__), "csrc", "layers_common.h")).read()
+    body = re.search(r"float tanh_rel\(float v\) \{(.*?)\n\}", text, re.S).group(1)
+    c = [float(a) / float(b) for a, b in re.findall(r"(-?\d+)\.0f / (\d+)", body.split("const float e")[0])]
+    v = np.linspace(1e-3, 0.5, 2001)
+    p = v + v * sum(k * v ** (2 * i + 2) for i, k in enumerate(c))
+    assert len(c) == 7 and np.abs(p / np.tanh(v) - 1).max() < 9e-9
+    body = re.search(r"float normal_tail\(float z, float\* e\) \{(.*?)\n\}", text, re.S).group(1)
+    c = [float(a) for a in re.findall(r"-?0\.\d{6,}(?=f)", body.split("const float p =")[1].split(";")[0])]
+    z = np.concatenate([np.linspace(0, 40, 40001), np.geomspace(40, 1e6, 2000)])
+    t = 1 / (1 + 0.356 * z / math.sqrt(2))
+    assert len(c) == 10 and np.abs(t * sum(k * t ** i for i, k in enumerate(c)) / (erfcx(z / math.sqrt(2)) / 2) - 1).max() < 4e-8
