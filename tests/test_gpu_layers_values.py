@@ -155,3 +155,110 @@ def test_group_norm_both_sides_of_one_launch(ctx, dtype, shape):
     n, r, c, G = shape
     x, gamma, beta = randn((n, r, c), DT[dtype], 1, 1.5, 0.7), randn((c,), torch.float32, 2, 0.3, 1.0), randn((c,), torch.float32, 3, 0.3)
     check_norm(ctx, x, gamma, beta, G, "swish", dy=randn((n, r, c), DT[dtype], 4))
+
+
+# ---- whole numbers: every sum is exact in 32 bits, so every result is the exact value rounded once, and one lost row or column shows ---------------------
+
+def ints(shape, dt, seed, hi=1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(-hi, hi + 1, shape, generator=g, device="cuda").to(dt)
+
+
+def exact_linear(ctx, x, w, bias, res, act, dy):
+    """x, w, dy, res, bias of whole numbers, act None or relu: bits of y, dx, dw, dbias"""
+    dt = x.dtype
+    y, pre = ctx.linear(x, w, bias, res, activation=act, want_preact=True)
+    z = x.double() @ w.double() + bias.double()
+    v = z.clamp(min=0) if act else z
+    assert torch.equal(y, (v + (0 if res is None else res.double())).to(dt))
+    dz = dy.double() * ((z > 0) if act else 1)
+    ref = ((dz @ w.double().t()).to(dt), (x.double().t() @ dz).to(dt), dz.sum(0).float())
+    for kept in ([pre, None] if pre is not None else [None]):
+        for got, want, name in zip(ctx.linear_backward(dy, x, w, kept, bias, activation=act), ref, ("dx", "dw", "dbias")):
+            assert torch.equal(got, want), (name, tuple(x.shape), tuple(w.shape), int((got != want).sum()))
+
+
+INT_SHAPES = [(2500, 64, 64), (4099, 64, 48), (30000, 64, 1), (30000, 50, 33), (4099, 24, 128), (2500, 128, 60), (2500, 177, 93), (9999, 256, 128), (4099, 300, 264),
+              (100, 5000, 60), (37, 70, 9000), (9999, 64, 640), (9984, 64, 640), (128, 6400, 640), (6400, 640, 128), (1, 1000, 999), (3, 999, 64), (8, 513, 77)]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", INT_SHAPES, ids=str)
+def test_linear_whole_numbers(ctx, dtype, shape):
+    m, k, n = shape
+    dt = DT[dtype]
+    for act in (None, "relu"):
+        exact_linear(ctx, ints((m, k), dt, 1), ints((k, n), dt, 2), ints((n,), torch.float32, 3, 3), ints((m, n), dt, 4) if n % 2 else None, act, ints((m, n), dt, 5))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(1000, 64, 64), (2500, 177, 93), (2500, 300, 264), (2560, 320, 1024), (6400, 640, 128)], ids=str)
+def test_linear_whole_numbers_in_rows_of_wider_arrays(ctx, dtype, shape):
+    """x, w, residual and dy as slices that start anywhere, at narrow, ordinary and wide sizes"""
+    m, k, n = shape
+    dt = DT[dtype]
+    for lo, act in ((0, None), (8, "relu"), (3, None), (5, "relu")):
+        x, w = ints((m, k + 24), dt, 1)[:, lo:lo + k], ints((k, n + 16), dt, 2)[:, lo:lo + n]
+        exact_linear(ctx, x, w, ints((n,), torch.float32, 3, 3), ints((m, n + 40), dt, 4)[:, lo:lo + n], act, ints((m, n + 8 + lo), dt, 5)[:, 8:8 + n])
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(1, 2500, 64, 8), (3, 4099, 40, 5), (2, 9999, 24, 2), (1, 30000, 8, 4), (1, 30001, 64, 8), (40, 784, 64, 8), (300, 33, 256, 32),
+                                   (1, 777, 1030, 5), (600, 2000, 8, 1)], ids=str)
+def test_group_norm_whole_numbers(ctx, dtype, shape):
+    """x is 1 and -1 in neighbouring channels: mean 0, variance 1 and, without eps, x itself normalised; dbeta and dgamma are whole sums"""
+    n, r, c, G = shape
+    dt = DT[dtype]
+    x = torch.ones((n, r, c), device="cuda")
+    x[..., 1::2] = -1
+    x = (x * (2 * ints((n, r, 1), torch.float32, 1).clamp(min=0) - 1)).to(dt)
+    y, st = ctx.group_norm(x, groups=G, eps=0.0, want_stats=True)
+    assert torch.equal(y, x) and not st[..., 0].any() and bool((st[..., 1] == 1).all())
+    dy = ints((n, r, c), dt, 2)
+    _, dg, db = ctx.group_norm_backward(dy, x, None, None, st)
+    assert torch.equal(db, dy.double().sum((0, 1)).float()) and torch.equal(dg, (dy.double() * x.double()).sum((0, 1)).float())
+    assert ctx.group_norm_backward(dy, x, None, None, st, want_dx=False)[1].equal(dg)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 29584, 512, 32), (1, 14000, 512, 512), (1, 3000, 4096, 32), (1, 3000, 2049, 2049)], ids=str)
+def test_group_norm_of_one_sample_with_many_groups(ctx, dtype, shape):
+    n, r, c, G = shape
+    x, gamma, beta = randn((n, r, c), DT[dtype], 1, 1.5, 0.7), randn((c,), torch.float32, 2, 0.3, 1.0), randn((c,), torch.float32, 3, 0.3)
+    check_norm(ctx, x, gamma, beta, G, "swish", dy=randn((n, r, c), DT[dtype], 4))
+
+
+# ---- autograd in every type, narrow and wide, on slices: the gradients of the explicit calls ---------------------------------------------------
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(64, 24), (64, 1), (200, 136)], ids=str)
+def test_autograd_gives_the_explicit_calls_gradients(ctx, dtype, shape):
+    k, n = shape
+    dt = DT[dtype]
+    wide = randn((2, 9, 31, k + 16), dt, 1)
+    for lo in (0, 3, 8):
+        x = wide[..., lo:lo + k].detach().requires_grad_()
+        w, bias = randn((k, n), dt, 2, k ** -0.5).requires_grad_(), randn((n,), torch.float32, 3, 0.3).requires_grad_()
+        gamma, beta = randn((k,), torch.float32, 4, 0.3, 1.0).requires_grad_(), randn((k,), torch.float32, 5).requires_grad_()
+        res = randn((2, 9, 31, n), dt, 6).requires_grad_()
+        dy = randn((2, 9, 31, n + 4), dt, 7)[..., 4:]
+        assert not x.is_contiguous()
+        h = ctx.group_norm(x, gamma, beta, groups=8, activation="swish")
+        y = ctx.linear(h, w, bias, residual=res, activation="tanh", scale=0.5)
+        y.backward(dy)
+        with torch.no_grad():
+            h2, st = ctx.group_norm(x, gamma, beta, groups=8, activation="swish", want_stats=True)
+            y2, pre = ctx.linear(h2, w, bias, residual=res, activation="tanh", scale=0.5, want_preact=True)
+            dh, dw, db = ctx.linear_backward(dy, h2, w, pre, bias, activation="tanh", scale=0.5)
+            dx, dg, dbe = ctx.group_norm_backward(dh, x, gamma, beta, st, activation="swish")
+        assert (pre is None) == (n != 136)
+        for got, want in ((y, y2), (x.grad, dx), (w.grad, dw), (bias.grad, db), (gamma.grad, dg), (beta.grad, dbe), (res.grad, dy)):
+            assert got.dtype == want.dtype and torch.equal(got, want)
+        # one leaf at a time: what is not wanted is not formed, the rest keeps its bits
+        for leaf, want in ((x, dx), (w, dw), (bias, db), (gamma, dg)):
+            a = {id(t): t.detach().clone() if t is not x else t.detach() for t in (x, w, bias, gamma, beta, res)}
+            a[id(leaf)].requires_grad_()
+            out = ctx.linear(ctx.group_norm(a[id(x)], a[id(gamma)], a[id(beta)], groups=8, activation="swish"), a[id(w)], a[id(bias)], residual=a[id(res)],
+                             activation="tanh", scale=0.5)
+            got, = torch.autograd.grad(out, a[id(leaf)], dy)
+            assert torch.equal(got, want)
