@@ -81,6 +81,8 @@ __device__ __forceinline__ void mma_block(f32x4 (&acc)[I][J], const typename Mma
 // after the other: rounded once instead, dx and dw were 1.4 times as far from their 64-bit values as their own rounding takes them (bf16 2.35e-3 against 1.66e-3).
 // The pair holds 16 (bf16) or 22 bits (fp16).  fp16 has a narrow range: the value is halved, so that a slope up to 1.13 does not overflow it, and its low
 // half, 11 bits further down, comes up by 2^11, out of the subnormals (smallest piece 2^-35).
+// relu's slope is 0 or 1: dz has the arrays' bits as it is, and a low half of 0 would turn the infinite dw of an infinite x into NaN.
+template <class T> inline bool dz_is_pair(int act) { return sizeof(T) == 2 && act != TTC_ACT_NONE && act != TTC_ACT_RELU; }
 template <class T> constexpr float DZ_DOWN = std::is_same_v<T, f16> ? 0.5f : 1.0f;      // undone by the products' alpha
 template <class T> constexpr float LO_UP = std::is_same_v<T, f16> ? 2048.0f : 1.0f;
 template <class T>
@@ -800,7 +802,7 @@ constexpr int NARROW_BWD_LDS() {
     return run > red ? run : red;
 }
 // FULL: cin and cout are exactly the padded sides and the preact is formed again (as in k_narrow: no masks, no second set of addresses).
-// PAIR: 16-bit with an activation; without one dz is dy itself, and the registers of z and of the pair are free.
+// PAIR: 16-bit with an activation but relu (dz_is_pair).
 template <class T, int KS, int NS, bool FULL, bool PAIR>
 __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) void k_narrow_bwd(NarrowBwd a) {
     constexpr int KP = KS * KSTEP<T>, NP = NS * KSTEP<T>, FK = KP / 16, FN = NP / 16;
@@ -858,7 +860,7 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
                 for (int s = 0; s < KS; ++s) x[h].v[s] = make_uint4(0, 0, 0, 0);
             }
             Frag dz[NS], dl[NS];                             // dl: the pair's low halves
-            if ((H16 && !PAIR) || (!H16 && a.act == TTC_ACT_NONE)) {
+            if (!PAIR && a.act == TTC_ACT_NONE) {
 #pragma unroll
                 for (int p = 0; p < NS; ++p) {
                     dz[p] = __builtin_bit_cast(Frag, d[h].v[p]);
@@ -895,14 +897,14 @@ __global__ __launch_bounds__(NT, KS * NS <= (sizeof(T) == 2 ? 4 : 8) ? 2 : 1) vo
                     float t[V], zz[V];
 #pragma unroll
                     for (int i = 0; i < V; ++i) { t[i] = (float)dv[i]; zz[i] = z[H16 ? 2 * p + i / 4 : p][0][i & 3]; }
-                    slope_vec<V>(t, zz, a.act);
+                    slope_vec<V>(t, zz, H16 && !PAIR ? TTC_ACT_RELU : a.act);
                     int cols = FULL ? V : a.N - p * KSTEP<T> - q * V;
                     if (!FULL) asm volatile("" : "+v"(cols));           // compared where it is used: as masks kept over the loop it is 16 registers
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         // a padded column: its zero weights make z NaN where x is infinite, and that times its zero dy would reach every dx of the row
                         if (!FULL && i >= cols) t[i] = 0.0f;
-                        t[i] *= DZ_DOWN<T>;
+                        if (PAIR) t[i] *= DZ_DOWN<T>;
                         db[p][i] += t[i];
                         if constexpr (PAIR) {
                             T hi, lo;
@@ -1070,7 +1072,7 @@ __global__ __launch_bounds__(NT) void k_dz(DzArgs a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) s[i] += d[i];
             if (!a.dz) continue;
-            if constexpr (sizeof(T) == 4) {
+            if (sizeof(T) == 4 || !a.lo) {
                 store_vec<T, V>((T*)a.dz + r * a.N + c0, d);
             } else {
                 T hi[V], lo[V];
@@ -1268,7 +1270,7 @@ BwdWs linear_ws(const ttc_linear_desc* d, bool have_z) {
     dz_geometry(z, col_vec(d->cout, dtype_bytes(d->dtype)), &w.blocks, &tiles);
     w.dz = act && !have_z ? up(cells * sizeof(float)) : 0;
     w.lo = w.dz + (act ? up(cells * dtype_bytes(d->dtype)) : 0);
-    w.sums = w.lo + (act && d->dtype != TTC_DT_F32 ? up(cells * 2) : 0);
+    w.sums = w.lo + (d->dtype != TTC_DT_F32 && dz_is_pair<f16>(d->activation) ? up(cells * 2) : 0);
     w.part = w.sums + up((size_t)w.blocks * d->cout * sizeof(float));
     const size_t zs = act && !have_z ? (size_t)gemm_splits(d->rows, d->cout, d->cin, dtype_bytes(d->dtype)) : 1;
     w.dx_splits = gemm_splits(d->rows, d->cin, d->cout, dtype_bytes(d->dtype));
@@ -1327,7 +1329,7 @@ hipError_t narrow_bwd_launch(const NarrowBwd& a, int blocks, hipStream_t s) {
             return launch(k_narrow_bwd<T, KS, NS, false, PAIR>, NARROW_BWD_LDS<T, KS, NS, PAIR>(), ragged);
         };
         if constexpr (sizeof(T) == 2)
-            if (a.act != TTC_ACT_NONE) return pick(std::true_type{});
+            if (dz_is_pair<T>(a.act)) return pick(std::true_type{});
         return pick(std::false_type{});
     };
     constexpr std::integral_constant<int, 2> two{};
@@ -1420,7 +1422,8 @@ ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void*
             return TTC_OK;
         }
         char* ws = (char*)d_ws;
-        const float alpha = d->scale / (act ? DZ_DOWN<T> : 1.0f);
+        const bool pair = dz_is_pair<T>(d->activation);
+        const float alpha = d->scale / (pair ? DZ_DOWN<T> : 1.0f);
         GemmArgs o{};                                        // dw [cin, cout], scaled where the splits are joined
         o.M = d->cin; o.N = d->cout; o.C = d_dw; o.ldc = d->cout; o.alpha = alpha;
         if (narrow_bwd(d)) {
@@ -1442,11 +1445,11 @@ ttc_status ttc_linear_backward(ttc_ctx* c, const ttc_linear_desc* d, const void*
             z = (const float*)ws;
         }
         const T* dz = act ? (const T*)(ws + w.dz) : (const T*)d_dy;     // without an activation dz is dy itself; the scale is in the epilogues either way
-        const void* dz_lo = act && sizeof(T) == 2 ? ws + w.lo : nullptr;
+        void* dz_lo = pair ? ws + w.lo : nullptr;
         const long dz_pitch = act ? d->cout : d->dy_pitch;
         if (act || d_dbias) {
             DzArgs q{};
-            q.dy = d_dy; q.z = z; q.dz = act && (d_dx || d_dw) ? ws + w.dz : nullptr; q.lo = ws + w.lo; q.part = d_dbias ? (float*)(ws + w.sums) : nullptr;
+            q.dy = d_dy; q.z = z; q.dz = act && (d_dx || d_dw) ? ws + w.dz : nullptr; q.lo = dz_lo; q.part = d_dbias ? (float*)(ws + w.sums) : nullptr;
             q.rows = d->rows; q.dpitch = d->dy_pitch; q.N = d->cout; q.act = d->activation;
             const int V = col_vec(d->cout, sizeof(T));
             int blocks, tiles;

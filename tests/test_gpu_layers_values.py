@@ -262,3 +262,23 @@ def test_autograd_gives_the_explicit_calls_gradients(ctx, dtype, shape):
                              activation="tanh", scale=0.5)
             got, = torch.autograd.grad(out, a[id(leaf)], dy)
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(100, 64, 64), (100, 64, 1), (101, 50, 33), (300, 200, 150), (3200, 512, 640)], ids=str)
+def test_linear_relu_weight_gradient_of_an_infinite_x(ctx, dtype, shape):
+    """inf * dz is an infinity of dz's sign, NaN where relu's slope or dy is 0; the other rows of dw are exact"""
+    m, k, n = shape
+    dt = DT[dtype]
+    x, w, dy, bias = ints((m, k), dt, 1), ints((k, n), dt, 2), ints((m, n), dt, 3), torch.zeros(n, device="cuda")
+    w[5] = w[5].abs() * 2 - 1                                     # the infinite element has weights 1 and -1
+    x[7, 5] = float("inf")
+    z = torch.cat([x[:7].double() @ w.double(), w[5:6].double() * float("inf"), x[8:].double() @ w.double()])
+    dz = dy.double() * (z > 0)
+    want = x.double().nan_to_num(posinf=0).t() @ dz
+    want[5] += float("inf") * dz[7]
+    _, pre = ctx.linear(x, w, bias, activation="relu", want_preact=True)
+    for kept in ([pre, None] if pre is not None else [None]):
+        dx, dw, db = ctx.linear_backward(dy, x, w, kept, bias, activation="relu")
+        assert torch.equal(dw.isnan(), want.isnan()) and torch.equal(dw.nan_to_num(), want.to(dt).nan_to_num())
+        assert torch.equal(dx, (dz @ w.double().t()).to(dt)) and torch.equal(db, dz.sum(0).float())
