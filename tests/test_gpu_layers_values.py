@@ -282,3 +282,41 @@ def test_linear_relu_weight_gradient_of_an_infinite_x(ctx, dtype, shape):
         dx, dw, db = ctx.linear_backward(dy, x, w, kept, bias, activation="relu")
         assert torch.equal(dw.isnan(), want.isnan()) and torch.equal(dw.nan_to_num(), want.to(dt).nan_to_num())
         assert torch.equal(dx, (dz @ w.double().t()).to(dt)) and torch.equal(db, dz.sum(0).float())
+
+
+# ---- offsets past 32 bits ----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cin,cout", [(64, 64), (64, 1), (264, 136)], ids=str)
+def test_linear_past_two_to_the_31_elements(ctx, cin, cout):
+    """x of more than 2^31 elements whose rows are zero but at both ends and next to the offsets of 2^31 elements and bytes"""
+    dt, m = torch.bfloat16, (1 << 31) // cin + 1003
+    x, dy = torch.zeros((m, cin), device="cuda", dtype=dt), torch.zeros((m, cout), device="cuda", dtype=dt)
+    at = [r for c in (0, (1 << 31) // cin, (1 << 30) // cin, (1 << 31) // max(cout, 64), (1 << 30) // max(cout, 64), m) for r in range(c - 20, c + 20) if 0 <= r < m]
+    at = torch.tensor(sorted(set(at)), device="cuda")
+    x[at], dy[at] = ints((len(at), cin), dt, 1), ints((len(at), cout), dt, 2)
+    w, bias = ints((cin, cout), dt, 3), torch.zeros(cout, device="cuda")
+    y, pre = ctx.linear(x, w, bias, activation="relu", want_preact=True)
+    z = x[at].double() @ w.double()
+    assert torch.equal(y[at], z.clamp(min=0).to(dt)) and int(torch.count_nonzero(y)) == int((z > 0).sum())
+    dx, dw, db = ctx.linear_backward(dy, x, w, pre, bias, activation="relu")
+    dz = dy[at].double() * (z > 0)
+    want = (dz @ w.double().t()).to(dt)
+    assert torch.equal(dx[at], want) and int(torch.count_nonzero(dx)) == int(torch.count_nonzero(want))
+    assert torch.equal(dw, (x[at].double().t() @ dz).to(dt)) and torch.equal(db, dz.sum(0).float())
+
+
+def test_group_norm_past_two_to_the_31_elements(ctx):
+    dt, n, r, c = torch.bfloat16, 3, (1 << 30) // 64 + 77, 64
+    x = torch.ones((n, r, c), device="cuda", dtype=dt)
+    x[..., 1::2] = -1
+    dy = torch.zeros_like(x)
+    at = torch.tensor([0, 1, 2, r - 3, r - 2, r - 1], device="cuda")
+    dy[:, at] = ints((n, 6, c), dt, 1)
+    y, st = ctx.group_norm(x, groups=8, eps=0.0, want_stats=True)
+    assert torch.equal(y, x)
+    del y
+    dx, dg, db = ctx.group_norm_backward(dy, x, None, None, st)
+    d = dy[:, at].double()
+    assert torch.equal(db, d.sum((0, 1)).float()) and torch.equal(dg, (d * x[:, at].double()).sum((0, 1)).float())
+    # the group means are at most 48 / 1.3e8, below what the type resolves next to 1; where dy is 0 they are what is left
+    assert bool(((dx[:, at].double() - d).abs() <= 1e-6).all()) and bool((dx.abs().amax(2).float()[:, 3:-3] <= 1e-6).all())
