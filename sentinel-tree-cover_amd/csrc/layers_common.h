@@ -43,8 +43,8 @@ __device__ __forceinline__ float tanh_rel(float v) {
 
 // h = normal distribution function of -|z|, and e = exp(-z^2 / 2).  h = erfc(x) / 2 with x = |z| / sqrt 2, and erfc(x) = exp(-x^2) t P(t),
 // t = 1 / (1 + 0.356 x): P is the degree-9 Chebyshev fit of exp(x^2) erfc(x) / t over t in (0, 1] (0.356 minimises its error; P is halved below):
-// with the rounded coefficients within 4e-8 of its value everywhere.  No 1 + erf: the negative tail keeps its relative accuracy.  A quarter of the registers of the library's erfc, which set
-// the kernels' occupancy.
+// with the rounded coefficients within 4e-8 of its value everywhere.  No 1 + erf: the negative tail keeps its relative accuracy.  A quarter of the registers
+// of the library's erfc, which set the kernels' occupancy.
 __device__ __forceinline__ float normal_tail(float z, float* e) {
     const float az = fabsf(z), t = __builtin_amdgcn_rcpf(1.0f + (0.356f * 0.70710678f) * az);
     const float p = 0.100425743f + t * (0.100426443f + t * (0.094032362f + t * (0.081815816f + t * (0.0595245f + t * (0.061009083f

@@ -6,7 +6,7 @@
 //
 // A product is C[i, j] = sum_c A(i, c) B(c, j), where each operand is stored either with the contracted index contiguous ("KC": x and dz in dx, w in dx) or
 // with its free index contiguous ("FC": w in y, x and dz in dw).  By size (host code at the end):
-//   k_narrow, k_narrow_bwd   up to 128 columns, weights in LDS: bound by the rows' bytes; the backward pass in one pass over the rows
+//   k_narrow, k_narrow_bwd   up to 128 columns, weights in LDS: bound by the rows' bytes forward in 16 bits; the backward pass in one pass over the rows
 //   k_few                    a few rows: bound by reading w
 //   k_gemm_wide              many 256 x 256 / 256 x 128 tiles of aligned rows: bound by the matrix cores
 //   k_gemm                   everything else; with few tiles the contracted index is split and k_join adds the parts
